@@ -174,6 +174,17 @@ int rte_embed_bwd_group(const int64_t* tokens, const float* dtable, int64_t* acc
 int rte_embed_bwd_grouped(const float* dx, float* dtable, int64_t* accum, int32_t n_tokens, int32_t d, int32_t vocab,
                           rte_stream_t stream);
 
+/* The operator table's lookup: out[i, :] = scale * table[ids[i], :], table [V, d] and out [n, d] of `type` (RTE_TYPE_*), both contiguous;
+ * an id out of range gives zeros and sets status.  Its gradient: dtable[v, :] = scale * the sum of dy[i, :] over ids[i] == v, in the
+ * order of i (fp32, rounded once; reproducible bit for bit), zeros in rows that no id names and in row padding_idx (< 0: none).
+ * scratch: rte_embedding_bwd_scratch(n, d) bytes on 16, any contents.  n <= RTE_EMBEDDING_MAX_TOKENS.                  */
+enum { RTE_EMBEDDING_MAX_TOKENS = 1 << 27 };
+int rte_embedding_fwd(const int64_t* ids, int64_t n, const void* table, int32_t type, int32_t V, int32_t d, float scale, void* out,
+                      int32_t* status, rte_stream_t stream);
+int64_t rte_embedding_bwd_scratch(int64_t n, int32_t d);
+int rte_embedding_bwd(const int64_t* ids, int64_t n, const void* dy, int32_t type, int32_t V, int32_t d, float scale,
+                      int64_t padding_idx, void* dtable, void* scratch, int64_t scratch_bytes, int32_t* status, rte_stream_t stream);
+
 /* ------------------------------------------------- RMSNorm (kernels/reference.py:9-17)
  * y = x * rsqrt(mean(x^2) + eps) * w [* (1 + film_gamma) + film_beta]  (FiLM: layers.py:841-847)
  * x f32 [rows,d]; y bf16 and/or f32 (either may be NULL); rstd f32 [rows] saved for backward.
@@ -288,6 +299,35 @@ int rte_ce_loss_lse(const void* logits, int32_t f32, int32_t ldl, const int64_t*
                     int32_t V, int32_t* status, rte_stream_t stream);
 int rte_ce_gradient(const void* logits, int32_t f32, int32_t ldl, const int64_t* targets, const float* row_weight, int32_t S,
                     const float* lse, void* dlogits, int32_t rows, int32_t V, int32_t* status, rte_stream_t stream);
+/* ------------------------------------------------ scores of tokens under rows of logits (no counterpart in the reference's table)
+ * logits [rows, V] of `type`, row stride ldl in elements (any, 0 too); V, top_k and k as stated, lists of at most RTE_TOKEN_LIST_MAX.
+ * Everything is taken of softmax(logits / temperature); -inf has probability zero, NaN or +inf make a row's results NaN.
+ * rte_token_logprobs_fwd: logprob f32 [rows] of tokens[row], entropy f32 [rows], the top_k largest as top_logprobs f32 / top_ids
+ *   int64 [rows, top_k] in descending order (equal logits: lower column first; NaN above all).  A row whose token is ignore_index (or
+ *   out of range, which sets status) is not read: zeros, ids -1.  A row of nothing but -inf: log probabilities -inf, entropy 0.
+ *   row_stats f32 [rows, 2] is kept for backward.
+ * rte_token_logprobs_bwd: dlogits [rows, V] contiguous, of `type`, from the gradients of logprob, entropy and top_logprobs (NULL: none);
+ *   zeros in rows without a token or a finite logit.
+ * rte_distill_topk_fwd: loss f32 [rows] = temperature^2 * KL(teacher || softmax(logits / temperature)).  The teacher's row is a list of
+ *   k log probabilities (teacher f32 [rows, k]) at ids int64 [rows, k]; a negative id is an unused slot (one >= V too, and sets status), an
+ *   id named twice counts with both.  tail = 0: the list is renormalised, so any constant may be added to a row; tail = 1: what it lacks
+ *   of one, max(0, 1 - sum), is the probability of all other tokens together (left out where the student gives them none).  A row
+ *   without a used slot or teacher probability (tail = 0) has loss and gradient zero and is not read.  row_stats f32 [rows, 8], on 16 bytes.
+ * rte_distill_topk_bwd: dlogits [rows, V] contiguous, of `type`, from dloss f32 [rows].                                            */
+enum { RTE_TYPE_BF16 = 0, RTE_TYPE_F32 = 1, RTE_TYPE_F16 = 2 };
+enum { RTE_TOKEN_LIST_MAX = 256 };
+int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t ldl, const int64_t* tokens, int64_t ignore_index, float temperature,
+                           int32_t top_k, float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, float* row_stats,
+                           int32_t rows, int32_t V, int32_t* status, rte_stream_t stream);
+int rte_token_logprobs_bwd(const void* logits, int32_t type, int64_t ldl, const int64_t* tokens, float temperature, int32_t top_k,
+                           const int64_t* top_ids, const float* row_stats, const float* entropy, const float* g_logprob,
+                           const float* g_entropy, const float* g_top, void* dlogits, int32_t rows, int32_t V, rte_stream_t stream);
+int rte_distill_topk_fwd(const void* logits, int32_t type, int64_t ldl, const float* teacher, const int64_t* ids, int32_t k,
+                         float temperature, int32_t tail, float* loss, float* row_stats, int32_t rows, int32_t V, int32_t* status,
+                         rte_stream_t stream);
+int rte_distill_topk_bwd(const void* logits, int32_t type, int64_t ldl, const float* teacher, const int64_t* ids, int32_t k,
+                         float temperature, const float* row_stats, const float* dloss, void* dlogits, int32_t rows, int32_t V,
+                         rte_stream_t stream);
 /* out[b] = sum_s in[b*S + s]  (per-sample loss sums, models.py:75) */
 int rte_segment_sum(const float* in, float* out, int32_t n_seg, int32_t seg_len, rte_stream_t stream);
 

@@ -17,6 +17,8 @@ ROUTER_MAX_R, ROUTER_MAX_K, ROUTER_MAX_T = 32, 8, 128
 ROUTER_DPOOLED_PARTS = 4
 ERR_ALIGNMENT, ERR_UNSUPPORTED = -2, -5
 ADAMW_CHUNK = 4096
+TYPE_BF16, TYPE_F32, TYPE_F16 = 0, 1, 2
+TOKEN_LIST_MAX, EMBEDDING_MAX_TOKENS = 256, 1 << 27
 
 
 class GemmArgs(C.Structure):
@@ -123,6 +125,9 @@ PROTOTYPES = {
     "rte_embed_bwd": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_vp, c_vp]),
     "rte_embed_bwd_group": (C.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_vp, c_vp]),
     "rte_embed_bwd_grouped": (C.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_vp]),
+    "rte_embedding_fwd": (C.c_int, [c_vp, c_i64, c_vp, c_i32, c_i32, c_i32, c_f32, c_vp, c_vp, c_vp]),
+    "rte_embedding_bwd_scratch": (c_i64, [c_i64, c_i32]),
+    "rte_embedding_bwd": (C.c_int, [c_vp, c_i64, c_vp, c_i32, c_i32, c_i32, c_f32, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp]),
     "rte_rmsnorm_fwd": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_f32, c_vp]),
     "rte_rmsnorm_bwd": (C.c_int, [c_vp] * 12 + [c_i32, c_i32, c_i32, P(c_i32), c_vp]),
     "rte_rmsnorm_bwd_splits": (C.c_int, [c_vp] * 6 + [c_i32, c_i64] + [c_vp] * 6 + [c_i32, c_i32, c_i32, P(c_i32), c_vp]),
@@ -141,6 +146,10 @@ PROTOTYPES = {
     "rte_ce_loss_lse": (C.c_int, [c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
     "rte_ce_gradient": (C.c_int, [c_vp, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
     "rte_ce_fwd_bwd": (C.c_int, [c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
+    "rte_token_logprobs_fwd": (C.c_int, [c_vp, c_i32, c_i64, c_vp, c_i64, c_f32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
+    "rte_token_logprobs_bwd": (C.c_int, [c_vp, c_i32, c_i64, c_vp, c_f32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp]),
+    "rte_distill_topk_fwd": (C.c_int, [c_vp, c_i32, c_i64, c_vp, c_vp, c_i32, c_f32, c_i32, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
+    "rte_distill_topk_bwd": (C.c_int, [c_vp, c_i32, c_i64, c_vp, c_vp, c_i32, c_f32, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp]),
     "rte_segment_sum": (C.c_int, [c_vp, c_vp, c_i32, c_i32, c_vp]),
     "rte_router_fwd": (C.c_int, [c_vp, P(RouterWeights), c_vp, P(RouterOut)] + [c_i32] * 9 + [c_vp]),
     "rte_router_aux_add_dh0": (C.c_int, [c_vp, c_vp] + [c_i32] * 6 + [c_vp]),

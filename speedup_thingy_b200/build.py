@@ -21,7 +21,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "lib" / "librte_b200.so"
 HOST_LIB = PKG / "lib" / "_rte_host.so"
 SOURCES = ["gemm_tcgen05.cu", "elementwise.cu", "attention.cu", "macro_phi.cu", "router.cu", "audit.cu", "shortlist.cu", "cluster_pool.cu", "svd_ffn.cu", "gemm_small.cu", "gemm_tile.cu", "gemm_resident.cu", "codebook.cu", "allreduce.cu", "host_random.cu",
-           "operator_table.cu"]
+           "operator_table.cu", "token_scores.cu", "embedding.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

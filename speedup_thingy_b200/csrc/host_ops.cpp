@@ -494,6 +494,132 @@ struct CrossEntropy : Function<CrossEntropy> {
 };
 Tensor cross_entropy(const Tensor& logits, const Tensor& targets) { return CrossEntropy::apply(logits, targets)[0]; }
 
+// --------------------------------------------------------------------------- scores of tokens under rows of logits
+int type_of(const Tensor& t) { return t.scalar_type() == BF ? RTE_TYPE_BF16 : t.scalar_type() == F32 ? RTE_TYPE_F32 : RTE_TYPE_F16; }
+
+struct Rows {                                 // [..., V] as rows of one stride: a view where the strides allow it, a copy elsewhere
+  Tensor t;
+  int64_t rows, V, ld;
+  explicit Rows(const Tensor& x) : t(x), V(x.size(-1)), ld(-1) {
+    rows = V ? x.numel() / V : 0;
+    int64_t upto = 0;                         // how many rows the dimensions looked at so far hold, and whether `ld` steps through them
+    bool even = x.stride(-1) == 1 || V == 1;
+    for (int64_t i = x.dim() - 2; i >= 0 && even; --i) {
+      if (x.size(i) == 1) continue;
+      if (ld < 0) { ld = x.stride(i); upto = x.size(i); }
+      else { even = x.stride(i) == ld * upto; upto *= x.size(i); }
+    }
+    if (!even) { t = x.contiguous(); ld = V; }
+    if (ld < 0) ld = V;
+  }
+};
+// The kernels take the number of rows as an int32.
+void count_fits(int64_t n, const char* what) { TORCH_CHECK_VALUE(n < (int64_t(1) << 31), what, ": ", n, " rows in one call"); }
+Tensor grad_f32(const Tensor& g) { return g.defined() ? g.to(F32).contiguous() : Tensor(); }
+
+struct TokenLogprobs : Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index) {
+    Dev dev(logits);
+    const Rows x(logits);
+    count_fits(x.rows, "k_token_logprobs");
+    const Tensor tok = tokens.to(torch::kInt64).contiguous();
+    std::vector<int64_t> top(tokens.sizes().begin(), tokens.sizes().end());
+    top.push_back(top_k);
+    const Tensor logprob = empty_as(tok, F32), entropy = empty_as(tok, F32), stats = empty({x.rows, 2}, F32, logits);
+    const Tensor top_lp = at::empty(top, tok.options().dtype(F32)), top_ids = at::empty(top, tok.options());
+    if (x.rows > 0)
+      check(rte_token_logprobs_fwd(ptr(x.t), type_of(x.t), x.ld, tok.data_ptr<int64_t>(), ignore_index, temperature, top_k, f32(logprob), f32(entropy), f32(top_lp),
+                                   top_ids.data_ptr<int64_t>(), f32(stats), x.rows, x.V, dev.status, dev.st),
+            "rte_token_logprobs_fwd");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, tok, stats, entropy, top_ids});
+    ctx->mark_non_differentiable({top_ids});
+    ctx->saved_data["top_k"] = top_k;
+    ctx->saved_data["temperature"] = temperature;
+    return {logprob, entropy, top_lp, top_ids};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    Dev dev(saved[0]);
+    const Rows x(saved[0]);
+    const auto top_k = ctx->saved_data["top_k"].toInt();
+    const Tensor gl = grad_f32(g[0]), gh = grad_f32(g[1]), gt = top_k > 0 ? grad_f32(g[2]) : Tensor();
+    const Tensor dx = at::empty(saved[0].sizes(), x.t.options());
+    if (x.rows > 0)
+      check(rte_token_logprobs_bwd(ptr(x.t), type_of(x.t), x.ld, saved[1].data_ptr<int64_t>(), ctx->saved_data["temperature"].toDouble(), top_k,
+                                   saved[4].data_ptr<int64_t>(), f32(saved[2]), f32(saved[3]), f32(gl), f32(gh), f32(gt), ptr(dx), x.rows, x.V, dev.st),
+            "rte_token_logprobs_bwd");
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index) {
+  auto out = TokenLogprobs::apply(logits, tokens, top_k, temperature, ignore_index);
+  return {out[0], out[1], out[2], out[3]};
+}
+
+struct DistillTopk : Function<DistillTopk> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature, bool tail) {
+    Dev dev(logits);
+    const Rows x(logits);
+    count_fits(x.rows, "k_distill_topk");
+    const auto k = ids.size(-1);
+    const Tensor t = teacher.to(F32).contiguous(), id = ids.to(torch::kInt64).contiguous();
+    const Tensor loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), t.options()), stats = empty({x.rows, 8}, F32, logits);
+    if (x.rows > 0)
+      check(rte_distill_topk_fwd(ptr(x.t), type_of(x.t), x.ld, f32(t), id.data_ptr<int64_t>(), k, temperature, tail, f32(loss), f32(stats), x.rows, x.V, dev.status,
+                                 dev.st),
+            "rte_distill_topk_fwd");
+    ctx->save_for_backward({logits, t, id, stats});
+    ctx->saved_data["temperature"] = temperature;
+    return {loss};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    Dev dev(saved[0]);
+    const Rows x(saved[0]);
+    const Tensor dloss = grad_f32(g[0]), dx = at::empty(saved[0].sizes(), x.t.options());
+    if (x.rows > 0)
+      check(rte_distill_topk_bwd(ptr(x.t), type_of(x.t), x.ld, f32(saved[1]), saved[2].data_ptr<int64_t>(), saved[2].size(-1),
+                                 ctx->saved_data["temperature"].toDouble(), f32(saved[3]), f32(dloss), ptr(dx), x.rows, x.V, dev.st),
+            "rte_distill_topk_bwd");
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor distill_topk(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature, bool tail) {
+  return DistillTopk::apply(logits, teacher.detach(), ids, temperature, tail)[0];
+}
+
+// --------------------------------------------------------------------------- embedding
+struct Embedding : Function<Embedding> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) {
+    Dev dev(weight);
+    const Tensor id = ids.to(torch::kInt64).contiguous(), w = weight.contiguous();
+    const auto n = id.numel(), V = w.size(0), d = w.size(1);
+    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+    shape.push_back(d);
+    const Tensor out = at::empty(shape, w.options());
+    if (n > 0) check(rte_embedding_fwd(id.data_ptr<int64_t>(), n, ptr(w), type_of(w), V, d, scale, ptr(out), dev.status, dev.st), "rte_embedding_fwd");
+    ctx->save_for_backward({id});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["dims"] = std::vector<int64_t>{V, d, padding_idx};
+    return {out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const Tensor id = ctx->get_saved_variables()[0], dy = g[0].contiguous();
+    Dev dev(dy);
+    const auto dims = ctx->saved_data["dims"].toIntVector();
+    const auto n = id.numel(), V = dims[0], d = dims[1];
+    const Tensor dw = empty({V, d}, dy.scalar_type(), dy);
+    if (n == 0) return {Tensor(), dw.zero_(), Tensor(), Tensor()};
+    const Tensor scratch = empty({rte_embedding_bwd_scratch(n, d)}, torch::kUInt8, dy);
+    check(rte_embedding_bwd(id.data_ptr<int64_t>(), n, ptr(dy), type_of(dy), V, d, ctx->saved_data["scale"].toDouble(), dims[2], ptr(dw), ptr(scratch),
+                            scratch.numel(), dev.status, dev.st),
+          "rte_embedding_bwd");
+    return {Tensor(), dw, Tensor(), Tensor()};
+  }
+};
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) { return Embedding::apply(ids, weight, scale, padding_idx)[0]; }
+
 // --------------------------------------------------------------------------- packed SwiGLU FFN
 struct PackedFfn : Function<PackedFfn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& wug, const Tensor& wdown) {
@@ -734,6 +860,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("matmul_oi", &matmul_oi);
   m.def("out_proj", &out_proj);
   m.def("cross_entropy", &cross_entropy);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("distill_topk", &distill_topk);
+  m.def("embedding", &embedding);
   m.def("packed_ffn", &packed_ffn);
   pybind11::class_<PoolModule>(m, "PoolModule")
       .def(pybind11::init<const std::map<std::string, Tensor>&, const std::map<std::string, int64_t>&>())

@@ -17,6 +17,8 @@ the input's dtype.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _abi as A
@@ -188,6 +190,87 @@ def k_cross_entropy_unreduced(logits, targets):
     if logits.shape[:-1] != targets.shape:
         raise ValueError("k_cross_entropy_unreduced: logits [..., V] with targets [...]")
     return _native(logits).cross_entropy(logits, targets)
+
+
+# --------------------------------------------------------------------------- scores of tokens under rows of logits
+_LOGIT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_ID_TYPES = (torch.int32, torch.int64)
+
+
+class TokenLogprobs(NamedTuple):
+    """Result of `k_token_logprobs`."""
+    logprob: torch.Tensor            # f32 [...]
+    entropy: torch.Tensor            # f32 [...]
+    top_logprobs: torch.Tensor       # f32 [..., top_k], descending
+    top_ids: torch.Tensor            # int64 [..., top_k]
+
+
+def _check_scores(name: str, logits, temperature, *others) -> None:
+    if logits.dtype not in _LOGIT_TYPES:
+        raise ValueError(f"{name}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    if logits.ndim == 0 or not 1 <= logits.shape[-1] < 2 ** 31:
+        raise ValueError(f"{name}: logits [..., V] with at least one column, got {tuple(logits.shape)}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"{name}: the temperature must be positive and finite, got {temperature}")
+    if any(t.device != logits.device for t in others):
+        raise ValueError(f"{name}: all tensors must be on {logits.device}")
+
+
+def k_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
+    """Log probability of `tokens` [...] under softmax(logits [..., V] / temperature), the rows' entropy (nats) and their `top_k`
+    (at most 256) most likely tokens, in one pass over the logits; statistics and results in fp32, logits bf16, fp16 or fp32.
+
+    Alternatives come in descending order of the logits, equal ones by the lower id.  Log probabilities (of the tokens and of the
+    alternatives) and entropies are differentiable.  Where a token is `ignore_index` the row is not read: zeros, ids -1, no gradient.  A
+    token outside the vocabulary is treated so too and noted in the status word (`CudaOps.check_status`).  Logits of -inf have
+    probability zero; a row of nothing else has log probabilities -inf, entropy 0 and no gradient.  Backward reads the logits again."""
+    _check_scores("k_token_logprobs", logits, temperature, tokens)
+    if tokens.dtype not in _ID_TYPES or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"k_token_logprobs: logits [..., V] with integer tokens [...], got {tuple(logits.shape)} with {tokens.dtype} {tuple(tokens.shape)}")
+    if not 0 <= top_k <= min(A.TOKEN_LIST_MAX, logits.shape[-1]):
+        raise ValueError(f"k_token_logprobs: top_k must be in 0..{min(A.TOKEN_LIST_MAX, logits.shape[-1])}, got {top_k}")
+    if 0 <= ignore_index < logits.shape[-1]:
+        raise ValueError(f"k_token_logprobs: ignore_index {ignore_index} is a token of the vocabulary")
+    _require_cuda_tensor(logits, tokens)
+    return TokenLogprobs(*_native(logits).token_logprobs(logits, tokens, int(top_k), float(temperature), int(ignore_index)))
+
+
+def k_distill_topk(logits, teacher_logprobs, teacher_ids, temperature: float = 1.0, tail: bool = False):
+    """Per-row loss temperature^2 * KL(teacher || softmax(logits [..., V] / temperature)) against a teacher of whom only a list is
+    kept: log probabilities [..., k] (k at most 256) at `teacher_ids` [..., k], both as `k_token_logprobs` with the same temperature
+    gives them.  `tail=False` renormalises the list (any constant may be added to a row, so the teacher's logits / temperature do as
+    well); `tail=True` keeps its probabilities and gives what they lack of one to all other tokens together.
+
+    Negative ids are unused slots (lists of uneven length), an id named twice counts with both of its entries, one outside the
+    vocabulary is unused too and noted in the status word.  A row without a used slot has loss and gradient zero and is not read.
+    Only the logits get a gradient; backward reads them again."""
+    _check_scores("k_distill_topk", logits, temperature, teacher_logprobs, teacher_ids)
+    if teacher_ids.dtype not in _ID_TYPES or not teacher_logprobs.is_floating_point():
+        raise ValueError(f"k_distill_topk: integer ids and floating log probabilities, got {teacher_ids.dtype} and {teacher_logprobs.dtype}")
+    if teacher_ids.shape != teacher_logprobs.shape or teacher_ids.ndim != logits.ndim or teacher_ids.shape[:-1] != logits.shape[:-1]:
+        raise ValueError(f"k_distill_topk: logits [..., V] with log probabilities and ids [..., k], got {tuple(logits.shape)}, "
+                         f"{tuple(teacher_logprobs.shape)}, {tuple(teacher_ids.shape)}")
+    if not 1 <= teacher_ids.shape[-1] <= A.TOKEN_LIST_MAX:
+        raise ValueError(f"k_distill_topk: lists of 1..{A.TOKEN_LIST_MAX} tokens, got {teacher_ids.shape[-1]}")
+    _require_cuda_tensor(logits, teacher_logprobs, teacher_ids)
+    return _native(logits).distill_topk(logits, teacher_logprobs, teacher_ids, float(temperature), bool(tail))
+
+
+# --------------------------------------------------------------------------- embedding
+def k_embedding(ids, weight, scale: float = 1.0, padding_idx: int | None = None):
+    """scale * weight[ids] over a table [V, d] in bf16, fp16 or fp32, rounded once; an id outside the table gives zeros and is noted in
+    the status word.  The table's gradient is dense: every row's sum in fp32 in the order of the tokens, so that it is the same bits
+    every time, rounded once; row `padding_idx` gets none."""
+    if weight.dtype not in _LOGIT_TYPES or weight.ndim != 2 or 0 in weight.shape or max(weight.shape) >= 2 ** 31 - 1:
+        raise ValueError(f"k_embedding: a table [V, d] in bf16, fp16 or fp32, got {weight.dtype} {tuple(weight.shape)}")
+    if ids.dtype not in _ID_TYPES or ids.numel() > A.EMBEDDING_MAX_TOKENS:
+        raise ValueError(f"k_embedding: at most {A.EMBEDDING_MAX_TOKENS} integer ids, got {ids.dtype} {tuple(ids.shape)}")
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"k_embedding: padding_idx must name a row of the table, got {padding_idx}")
+    if ids.device != weight.device:
+        raise ValueError(f"k_embedding: all tensors must be on {weight.device}")
+    _require_cuda_tensor(ids, weight)
+    return _native(weight).embedding(ids, weight, float(scale), -1 if padding_idx is None else int(padding_idx))
 
 
 # --------------------------------------------------------------------------- host-side helpers of the table
