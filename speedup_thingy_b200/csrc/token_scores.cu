@@ -10,226 +10,811 @@
 // Logits of the type's lowest value are ordinary numbers; -inf has probability zero and adds nothing to H.  A row of nothing but -inf
 // has no distribution: log probabilities -inf, H = 0, no gradient.  NaN or +inf make a row's results NaN.
 
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "rte_common.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace {
 
-constexpr int TS_THREADS = 256;
 constexpr int TS_MAX_LIST = RTE_TOKEN_LIST_MAX;
-constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
+constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
+constexpr float LN2 = 0.693147180559945309f;
+constexpr double LOG2E = 1.44269504088896340736, LN2_D = 0.693147180559945309417;
+constexpr float FAR = 1e36f;                   // exponents (in powers of two) beyond this are formed the careful way
 
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ float exp2_fast(float t) {            // two units in the last place, 0 below -126
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
 
-// Order of the alternatives: value, NaN above all, then the lower column.  Larger keys come first; 0 is below and ~0 above every key.
-__device__ __forceinline__ unsigned long long order_key(float v, int column) {
+// ---------------------------------------------------------------- 16 bytes of a row
+template <typename T> struct Vec;              // N values; pairs() takes them two at a time
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static constexpr uint32_t NONE = 0xff800000u;                  // -inf
+  static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[4]) {
+    x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ float max(const uint4& r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+  static __device__ __forceinline__ float to_f(float v) { return v; }
+  static __device__ __forceinline__ float from_f(float v) { return v; }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static constexpr uint32_t NONE = 0xff80ff80u;
+  static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  static __device__ __forceinline__ float max(const uint4& r) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    return make_uint4(rte::pack_bf16x2(x[0], x[1]), rte::pack_bf16x2(x[2], x[3]), rte::pack_bf16x2(x[4], x[5]), rte::pack_bf16x2(x[6], x[7]));
+  }
+  static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Vec<__half> {
+  static constexpr int N = 8;
+  static constexpr uint32_t NONE = 0xfc00fc00u;
+  static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[8]) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 f = __half22float2(h[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+  }
+  static __device__ __forceinline__ float max(const uint4& r) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint4 r;
+    __half2* h = reinterpret_cast<__half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    return r;
+  }
+  static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+};
+
+// A row as 16-byte pieces: piece v holds the columns [v * N - off, (v + 1) * N - off), so that all but the first and the last lie
+// whole inside the row, on 16 bytes.  Columns outside the row read as -inf.
+template <typename T>
+struct Row {
+  static constexpr int N = Vec<T>::N;
+  const T* x;
+  int V, off, pieces;
+  __device__ __forceinline__ Row(const T* row, int V_) : x(row), V(V_), off(int(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T)), pieces((V_ + off + N - 1) / N) {}
+  __device__ __forceinline__ int column(int v) const { return v * N - off; }
+  __device__ __forceinline__ bool whole(int v) const { const int c = column(v); return c >= 0 && c + N <= V; }
+  __device__ __forceinline__ uint4 load(int v) const {
+    const int c = column(v);
+    if (c >= 0 && c + N <= V) return __ldg(reinterpret_cast<const uint4*>(x + c));
+    uint4 r = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+    T* t = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (c + i >= 0 && c + i < V) t[i] = x[c + i];
+    return r;
+  }
+  __device__ __forceinline__ float at(int column) const { return Vec<T>::to_f(x[column]); }
+};
+
+// ---------------------------------------------------------------- sums of exponentials
+// Exponents are kept in powers of two relative to R = max * c, c = log2(e) / T: t = x c - R in one fused step, whose rounded R shifts
+// every t of a row alike and is taken out again at the end.  R >= -FAR: all logits at the type's lowest value (or -inf) add nothing
+// then.  A row whose own R is beyond FAR (the type's ends at small temperatures, rows of nothing but lowest values) is summed again
+// relative to its maximum, t = (x - max) c.
+struct Sums { float top, R, s, e; };           // largest logit, reference, sum of 2^t, sum of t 2^t
+__device__ __forceinline__ Sums no_sums() { return {-INFINITY, -FAR, 0.f, 0.f}; }
+__device__ __forceinline__ void move_to(Sums& a, float R) {      // the same sums relative to R >= a.R
+  const float d = a.R - R, f = exp2_fast(d);
+  a.e = f * (a.e + d * a.s);
+  a.s *= f;
+  a.R = R;
+}
+__device__ __forceinline__ float weighted(float t) { return fmaxf(t, -1e4f); }       // (t 2^t is 0 where t = -inf)
+
+template <int NT>
+__device__ __forceinline__ Sums block_sums(Sums a, Sums* red) {  // red: NT / 32 of them in shared memory; every thread gets the result
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (q == 1) {
+      if (NT == 32) break;
+      __syncthreads();
+      if (lane == 0) red[warp] = a;
+      __syncthreads();
+      a = lane < NT / 32 ? red[lane] : no_sums();
+    }
+    move_to(a, rte::warp_max(a.R));
+    a.top = rte::warp_max(a.top);
+    a.s = rte::warp_sum(a.s);
+    a.e = rte::warp_sum(a.e);
+  }
+  return a;
+}
+__device__ __forceinline__ bool careful(const Sums& a) { return a.top != -INFINITY && fabsf(a.R) >= FAR; }
+
+// What a row's sums say, in 64 bits: they are single values, and losses are small differences of them.
+struct RowSum {
+  double top, ln_s, shift;                     // ln of sum exp((x - top) / T); log2 of what the stored sum is too large by
+  __device__ __forceinline__ RowSum(const Sums& a, float c) : top(a.top) {
+    shift = careful(a) || !(fabsf(a.R) < FAR) ? 0. : (double)a.top * c - a.R;
+    ln_s = log((double)a.s) - shift * LN2_D;
+  }
+  __device__ __forceinline__ double logprob(float x, double inv_t) const { return (x - top) * inv_t - ln_s; }
+};
+
+// The exponent of a logit relative to the row's largest, as forward formed it; p = 2^(t - l2) with l2 as forward kept it.
+struct Exponent {
+  float top, c, R;
+  bool far;
+  __device__ __forceinline__ Exponent(float top_, float c_) : top(top_), c(c_), R(fmaxf(top_ * c_, -FAR)) { far = !(fabsf(R) < FAR); }
+  __device__ __forceinline__ float operator()(float x) const { return far ? (x - top) * c : fmaf(x, c, -R); }
+};
+
+// ---------------------------------------------------------------- the largest logits of a row
+// Order of the alternatives: value, NaN above all, then the lower column.  Larger keys come first.
+__device__ __forceinline__ uint32_t value_key(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);                            // (-0 = 0)
-  const uint32_t u = v != v ? 0xfffffffeu : (b & 0x80000000u ? ~b : b | 0x80000000u);
-  return (unsigned long long)u << 32 | (uint32_t)~column;
+  return v != v ? 0xfffffffeu : (b & 0x80000000u ? ~b : b | 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long order_key(float v, int column) { return (unsigned long long)value_key(v) << 32 | (uint32_t)~column; }
+__device__ __forceinline__ float key_value(unsigned long long key) {
+  const uint32_t u = uint32_t(key >> 32);
+  return u == 0xfffffffeu ? __uint_as_float(0x7fffffffu) : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(TS_THREADS)
-token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float inv_t, int k, float* __restrict__ logprob,
-                      float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids, float2* __restrict__ stats, int V, int* status) {
-  rte::after_previous_grid();
-  __shared__ float red[32];
-  __shared__ unsigned long long best[32];
-  const long long row = blockIdx.x, tok = tokens[row];
+// Candidates are what reaches a bound that at least k logits reach: the first tile's bound is the k-th largest of its 16-byte pieces'
+// maxima, later ones are the k-th largest candidate.  k + a few candidates pass in a tile of unordered logits.
+template <int NT, int U>
+struct TopK {
+  static constexpr int CAP = 2048;                       // candidates kept (the largest list and a warp's tile of pieces fit more than once)
+  static constexpr int PIECES = NT * U;
+  unsigned long long cand[CAP];
+  unsigned long long list[TS_MAX_LIST];
+  uint32_t piece_max[PIECES];
+  unsigned long long bound;
+  int count, held, listed;
+};
+
+// The largest bound that at least k (at most k + slack, unless equal keys forbid) of n keys reach; one warp, keys `step` words apart.
+__device__ uint32_t warp_bound(const uint32_t* keys, int n, int step, int k, int slack, int* reach) {
+  const int lane = threadIdx.x & 31;
+  uint32_t lo = 0xffffffffu, hi = 0;
+  for (int i = lane; i < n; i += 32) { lo = min(lo, keys[i * step]); hi = max(hi, keys[i * step]); }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi) + 1;           // (no key is ~0)
+  int at_lo = n;
+  while (hi - lo > 1 && at_lo > k + slack) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    int c = 0;
+    for (int i = lane; i < n; i += 32) c += keys[i * step] >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= k) { lo = mid; at_lo = c; } else hi = mid;
+  }
+  *reach = at_lo;
+  return lo;
+}
+
+// The k-th largest candidate (0: there are no more than k), by one warp.
+__device__ unsigned long long warp_kth(const unsigned long long* cand, int n, int k) {
+  if (n <= k) return 0;
+  const int lane = threadIdx.x & 31;
+  int reach;
+  const uint32_t value = warp_bound(reinterpret_cast<const uint32_t*>(cand) + 1, n, 2, k, 0, &reach);
+  if (reach == k) return (unsigned long long)value << 32;
+  int above = 0;                                         // equal values at the end of the list: the lowest columns
+  for (int i = lane; i < n; i += 32) above += uint32_t(cand[i] >> 32) > value;
+  const int want = k - __reduce_add_sync(0xffffffffu, above);
+  uint32_t lo = 0, hi = 0xffffffffu;                     // (column 0 has the key ~0: reached by `lo` alone)
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    int c = 0;
+    for (int i = lane; i < n; i += 32) c += uint32_t(cand[i] >> 32) == value && uint32_t(cand[i]) >= mid;
+    if (__reduce_add_sync(0xffffffffu, c) >= want) lo = mid; else hi = mid;
+  }
+  int c = 0;
+  for (int i = lane; i < n; i += 32) c += uint32_t(cand[i] >> 32) == value && uint32_t(cand[i]) >= hi;
+  if (__reduce_add_sync(0xffffffffu, c) >= want) lo = hi;
+  return (unsigned long long)value << 32 | lo;
+}
+
+// list = the k largest of the first n candidates (all of them if there are no more), in any order; `listed` of them; `bound`: the last.
+template <typename S, int NT>
+__device__ void select(S& S_, int n, int k) {
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const unsigned long long b = warp_kth(S_.cand, n, k);
+    if (threadIdx.x == 0) { S_.bound = b; S_.listed = 0; }
+  }
+  __syncthreads();
+  const unsigned long long b = S_.bound;
+  for (int i = threadIdx.x; i < n; i += NT)
+    if (S_.cand[i] >= b) S_.list[atomicAdd(&S_.listed, 1)] = S_.cand[i];
+  __syncthreads();
+}
+
+// Adds a tile's pieces (raw[u]: piece first + u * NT of the row) to the candidates.  `looked`: this thread's pieces may hold a NaN.
+template <typename T, int NT, int U>
+__device__ __forceinline__ void collect(TopK<NT, U>& S, const Row<T>& row, const uint4 (&raw)[U], const float (&top)[U], int first, int end, int k, bool start, bool looked) {
+  constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x;
+  if (start) {
+    int have = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = first + u * NT < end;
+      S.piece_max[u * NT + tid] = in ? value_key(top[u]) : 0;
+      have += in;
+    }
+    if (tid == 0) { S.count = 0; S.held = TopK<NT, U>::CAP; }
+    __syncthreads();
+    if (tid < 32) {
+      const int n = min(max(end - (first - tid), 0), NT * U);          // the pieces of the tile, one after the other
+      int reach;
+      const uint32_t b = n > k ? warp_bound(S.piece_max, n, 1, k, k / 8, &reach) : 0;
+      if (tid == 0) S.bound = (unsigned long long)b << 32;
+    }
+    __syncthreads();
+  }
+  uint32_t todo = 0;
+  {
+    const uint32_t bound = uint32_t(S.bound >> 32);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + u * NT < end && (looked || value_key(top[u]) >= bound)) todo |= 1u << u;
+  }
+  while (true) {
+    const unsigned long long bound = S.bound;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!(todo >> u & 1)) continue;
+      float x[N];
+      Vec<T>::unpack(raw[u], x);
+      const int c = row.column(first + u * NT);
+      uint32_t pass = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c + i >= 0 && c + i < row.V && order_key(x[i], c + i) >= bound) pass |= 1u << i;
+      const int n = __popc(pass);
+      if (n == 0) { todo &= ~(1u << u); continue; }
+      int at = atomicAdd(&S.count, n);
+      if (at + n > TopK<NT, U>::CAP) { atomicMin(&S.held, at); continue; }
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (pass >> i & 1) S.cand[at++] = order_key(x[i], c + i);
+      todo &= ~(1u << u);
+    }
+    if (!__syncthreads_or(todo)) break;
+    // full: only the k largest stay, and the rest of the tile has to reach the last of them
+    select<TopK<NT, U>, NT>(S, S.held, k);
+    const int n = S.listed;
+    for (int i = tid; i < n; i += NT) S.cand[i] = S.list[i];
+    if (tid == 0) { S.count = n; S.held = TopK<NT, U>::CAP; }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- one pass over a row's pieces [begin, end)
+// OUTSIDE: the columns of `id` (-1: none) are left out; `bits`: a bit per column of a tile, in shared memory.
+template <typename T, int NT, int U, bool ENTROPY, bool OUTSIDE>
+__device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, float c, int k, TopK<NT, U>* top_k, const int* id, int ids, uint32_t* bits) {
+  constexpr int N = Vec<T>::N, TILE = NT * U;
+  const int tid = threadIdx.x;
+  Sums a = no_sums();
+  for (int tile = begin; tile < end; tile += TILE) {
+    const int first = tile + tid;
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      raw[u] = first + u * NT < end ? row.load(first + u * NT) : make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+    if (OUTSIDE) {
+      __syncthreads();
+      for (int i = tid; i < TILE * N / 32; i += NT) bits[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < ids; i += NT) {
+        const int at = id[i] + row.off - tile * N;               // (id -1 lies before every tile's first column or is masked by the test)
+        if (id[i] >= 0 && at >= 0 && at < TILE * N) atomicOr(&bits[at >> 5], 1u << (at & 31));
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t listed = bits[(u * NT + tid) * N / 32] >> ((u * NT + tid) * N % 32) & ((1u << N) - 1);
+        if (listed) {
+          uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const uint32_t mask = N == 4 ? 0xffffffffu : i % 2 ? 0xffff0000u : 0x0000ffffu;
+            if (listed >> i & 1) w[i * 4 / N] = (w[i * 4 / N] & ~mask) | (Vec<T>::NONE & mask);
+          }
+          raw[u] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+    float top[U], all = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) { top[u] = Vec<T>::max(raw[u]); all = fmaxf(all, top[u]); }
+    if (all > a.top) {
+      a.top = all;
+      const float R = fmaxf(a.R, all * c);
+      if (ENTROPY) move_to(a, R);
+      else { a.s *= exp2_fast(a.R - R); a.R = R; }
+    }
+    const float negR = -a.R;
+    float s[2] = {0.f, 0.f}, e[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[N];
+      Vec<T>::unpack(raw[u], x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float t = fmaf(x[i], c, negR), p = exp2_fast(t);
+        s[i & 1] += p;
+        if (ENTROPY) e[i & 1] = fmaf(p, weighted(t), e[i & 1]);
+      }
+    }
+    s[0] += s[1];
+    a.s += s[0];
+    if (ENTROPY) a.e += e[0] + e[1];
+    if (k > 0) collect<T, NT, U>(*top_k, row, raw, top, first, end, k, tile == begin, s[0] != s[0]);
+  }
+  return a;
+}
+
+// The sums of a row whose reference is out of range (`careful`): relative to its largest logit, which is not -inf.
+template <typename T, int NT, bool OUTSIDE>
+__device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, float top, float c, const int* id, int ids, Sums* red) {
+  float s = 0.f, e = 0.f;
+  for (int j = max(row.column(begin), 0) + (int)threadIdx.x; j < min(row.column(end), row.V); j += NT) {
+    bool out = false;
+    if (OUTSIDE) for (int i = 0; i < ids; ++i) out |= id[i] == j;
+    if (out) continue;
+    const float t = (row.at(j) - top) * c, p = exp2_fast(t);
+    s += p;
+    e = fmaf(p, weighted(t), e);
+  }
+  Sums a = {top, 0.f, s, e};
+  a = block_sums<NT>(a, red);
+  a.R = copysignf(FAR, top);
+  return a;
+}
+
+// ---------------------------------------------------------------- forward
+// A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.
+template <typename T, int NT, int U>
+__global__ void __launch_bounds__(NT)
+token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, double inv_t, int k, float* __restrict__ logprob,
+                      float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids, float2* __restrict__ stats, int V, int C, int* status) {
+  rte::after_previous_grid();
+  extern __shared__ __align__(16) unsigned char dyn[];
+  TopK<NT, U>* top = reinterpret_cast<TopK<NT, U>*>(dyn);       // (there is none where k = 0)
+  __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
+  __shared__ Sums mine;
+  const long long row_at = blockIdx.x / C;
+  const int rank = blockIdx.x % C, tid = threadIdx.x;
+  const long long tok = tokens[row_at];
   if (tok < 0 || tok >= V) {
-    if (tok != ignore && status && tid == 0) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
-    if (tid == 0) { logprob[row] = 0.f; entropy[row] = 0.f; stats[row] = make_float2(0.f, 0.f); }
-    for (int i = tid; i < k; i += TS_THREADS) { top_lp[row * k + i] = 0.f; top_ids[row * k + i] = -1; }
+    if (rank == 0) {
+      if (tok != ignore && status && tid == 0) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
+      if (tid == 0) { logprob[row_at] = 0.f; entropy[row_at] = 0.f; stats[row_at] = make_float2(0.f, -INFINITY); }
+      for (int i = tid; i < k; i += NT) { top_lp[row_at * k + i] = 0.f; top_ids[row_at * k + i] = -1; }
+    }
     return;
   }
-  const T* x = logits + row * ld;
-  float m = -INFINITY;
-  for (int j = tid; j < V; j += TS_THREADS) m = fmaxf(m, to_f(x[j]));
-  m = rte::block_max(m, red);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float s = 0.f, e1 = 0.f;
-  for (int j = tid; j < V; j += TS_THREADS) {
-    const float d = (to_f(x[j]) - ref) * inv_t, e = expf(d);
-    s += e;
-    e1 += e == 0.f ? 0.f : e * d;
+  const Row<T> row(logits + row_at * ld, V);
+  float target = 0.f;
+  if (rank == 0 && tid == 0) target = row.at((int)tok);
+  const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
+  Sums a = stream<T, NT, U, true, false>(row, begin, end, c, k, top, nullptr, 0, nullptr);
+  a = block_sums<NT>(a, red);
+  if (k > 0) {
+    if (begin < end) select<TopK<NT, U>, NT>(*top, top->count, k);
+    else if (tid == 0) top->listed = 0;
   }
-  s = rte::block_sum(s, red);
-  e1 = rte::block_sum(e1, red);
-  const float ln_s = logf(s);
+  if (C > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) mine = a;
+    cluster.sync();
+    a = no_sums();
+    for (int r = 0; r < C; ++r) {
+      Sums b = *cluster.map_shared_rank(&mine, r);
+      const float R = fmaxf(a.R, b.R);
+      move_to(a, R);
+      move_to(b, R);
+      a.top = fmaxf(a.top, b.top);
+      a.s += b.s;
+      a.e += b.e;
+    }
+    if (careful(a)) {                                            // (all CTAs of the cluster see the same sums)
+      const Sums b = sums_far<T, NT, false>(row, begin, end, a.top, c, nullptr, 0, red);
+      cluster.sync();
+      if (tid == 0) mine = b;
+      cluster.sync();
+      a = b;
+      a.s = a.e = 0.f;
+      for (int r = 0; r < C; ++r) { const Sums* o = cluster.map_shared_rank(&mine, r); a.s += o->s; a.e += o->e; }
+    }
+    if (k > 0 && rank == 0) {
+      int n = 0;
+      for (int r = 0; r < C; ++r) {
+        const TopK<NT, U>* o = cluster.map_shared_rank(top, r);
+        const int m = o->listed;
+        for (int i = tid; i < m; i += NT) top->cand[n + i] = o->list[i];
+        n += m;
+      }
+      cluster.sync();                                            // (the others leave)
+      select<TopK<NT, U>, NT>(*top, n, k);
+    } else {
+      cluster.sync();
+    }
+    if (rank != 0) return;
+  } else if (careful(a)) {
+    a = sums_far<T, NT, false>(row, begin, end, a.top, c, nullptr, 0, red);
+  }
+  const bool none = a.s == 0.f;                                  // nothing but -inf
+  const RowSum sum(a, c);
   if (tid == 0) {
-    logprob[row] = s == 0.f ? -INFINITY : (to_f(x[tok]) - ref) * inv_t - ln_s;
-    entropy[row] = s == 0.f ? 0.f : ln_s - e1 / s;
-    stats[row] = make_float2(ref, ln_s);
+    logprob[row_at] = none ? -INFINITY : (float)sum.logprob(target, inv_t);
+    // H = ln s - sum t 2^t / s, relative to the same R
+    entropy[row_at] = none ? 0.f : LN2 * (log2f(a.s) - a.e / a.s);
+    stats[row_at] = make_float2(a.top, none ? -INFINITY : log2f(a.s));
   }
-  unsigned long long last = ~0ull;
-  for (int i = 0; i < k; ++i) {
-    unsigned long long mine = 0;
-    for (int j = tid; j < V; j += TS_THREADS) {
-      const unsigned long long key = order_key(to_f(x[j]), j);
-      if (key < last && key > mine) mine = key;
-    }
-    for (int o = 16; o > 0; o >>= 1) { const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, o); mine = other > mine ? other : mine; }
-    __syncthreads();
-    if ((tid & 31) == 0) best[tid >> 5] = mine;
-    __syncthreads();
-    for (int w = 0; w < TS_THREADS / 32; ++w) mine = best[w] > mine ? best[w] : mine;
-    last = mine;
-    if (tid == 0) {
-      const int j = (int)~(uint32_t)mine;
-      top_ids[row * k + i] = j;
-      top_lp[row * k + i] = s == 0.f ? -INFINITY : (to_f(x[j]) - ref) * inv_t - ln_s;
-    }
+  for (int i = tid; i < k; i += NT) {                            // the list's order: how many keys are larger
+    const unsigned long long key = top->list[i];
+    int before = 0;
+    for (int j = 0; j < k; ++j) before += top->list[j] > key;
+    top_ids[row_at * k + before] = (int)~(uint32_t)key;
+    top_lp[row_at * k + before] = none ? -INFINITY : (float)sum.logprob(key_value(key), inv_t);
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(TS_THREADS)
-token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, float inv_t, int k, const int64_t* __restrict__ top_ids,
-                          const float2* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ g_lp, const float* __restrict__ g_h,
-                          const float* __restrict__ g_top, T* __restrict__ dlogits, int V) {
-  rte::after_previous_grid();
-  const long long row = blockIdx.x, tok = tokens[row];
-  const float2 st = stats[row];
-  T* dx = dlogits + row * V;
-  const int tid = threadIdx.x;
-  if (tok < 0 || tok >= V || st.y == -INFINITY) {
-    for (int j = tid; j < V; j += TS_THREADS) dx[j] = from_f<T>(0.f);
-    return;
-  }
-  const T* x = logits + row * ld;
-  const float g = g_lp ? g_lp[row] : 0.f, gh = g_h ? g_h[row] : 0.f, H = entropy[row];
-  float all = g;
-  if (g_top) for (int i = 0; i < k; ++i) all += g_top[row * k + i];
-  for (int j = tid; j < V; j += TS_THREADS) {
-    const float lp = (to_f(x[j]) - st.x) * inv_t - st.y, p = expf(lp);
-    float d = p == 0.f ? 0.f : -p * (all + gh * (lp + H));
-    if (j == tok) d += g;
-    if (g_top) for (int i = 0; i < k; ++i) if (top_ids[row * k + i] == j) d += g_top[row * k + i];
-    dx[j] = from_f<T>(d * inv_t);
-  }
+template <int NT>
+__device__ __forceinline__ double block_sum_double(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (NT == 32) return v;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < NT / 32; ++w) v += red[w];
+  return v;
+}
+template <int NT>
+__device__ __forceinline__ float block_max_float(float v, float* red) {
+  v = rte::warp_max(v);
+  if (NT == 32) return v;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  for (int w = 0; w < NT / 32; ++w) v = fmaxf(v, red[w]);
+  return v;
 }
 
-// stats of a row, eight floats: max, ln s, coefficient of p outside the list, M (0: no gradient), the list's max, ln of its sum
-template <typename T>
-__global__ void __launch_bounds__(TS_THREADS)
-distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float temp, int tail,
-                    float* __restrict__ loss, float4* __restrict__ stats, int V, int* status) {
+// stats of a row, eight floats: largest logit, log2 of the sum, coefficient of p outside the list, M (0: no gradient), the list's
+// max, ln of its sum
+template <typename T, int NT, int U, bool TAIL>
+__global__ void __launch_bounds__(NT)
+distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, double temp,
+                    float* __restrict__ loss, float4* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
-  __shared__ float red[32];
   __shared__ int id[TS_MAX_LIST];
-  const long long row = blockIdx.x;
-  const int tid = threadIdx.x;
+  __shared__ float listed[TS_MAX_LIST];                          // the student's logits on the list
+  __shared__ uint32_t bits[TAIL ? NT * U * Vec<T>::N / 32 : 1];
+  __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
+  __shared__ double red_d[NT / 32 > 0 ? NT / 32 : 1];
+  __shared__ float red_f[NT / 32 > 0 ? NT / 32 : 1];
+  __shared__ Sums mine;
+  const long long row_at = blockIdx.x / C;
+  const int rank = blockIdx.x % C, tid = threadIdx.x;
+  const float* t = teacher + row_at * k;
+  const Row<T> row(logits + row_at * ld, V);
   bool any = false;
-  for (int i = tid; i < k; i += TS_THREADS) {
-    const long long v = ids[row * k + i];
+  float tmax = -INFINITY;
+  for (int i = tid; i < k; i += NT) {
+    const long long v = ids[row_at * k + i];
     if (v >= V && status) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
     id[i] = v < 0 || v >= V ? -1 : (int)v;
-    any |= id[i] >= 0;
+    if (id[i] < 0) continue;
+    any |= TAIL || t[i] != -INFINITY;
+    tmax = fmaxf(tmax, t[i]);
+    listed[i] = row.at(id[i]);
   }
   any = __syncthreads_or(any);
-  double tmax = -INFINITY, tsum = 0;
-  if (any && !tail) {
-    any = false;
-    for (int i = 0; i < k; ++i) {
-      if (id[i] < 0) continue;
-      tmax = fmax(tmax, (double)teacher[row * k + i]);
-      any |= teacher[row * k + i] != -INFINITY;
-    }
-    for (int i = 0; i < k; ++i) if (id[i] >= 0) tsum += exp(teacher[row * k + i] - tmax);
-  }
-  if (!any) {
-    if (tid == 0) { loss[row] = 0.f; stats[row * 2] = stats[row * 2 + 1] = make_float4(0.f, 0.f, 0.f, 0.f); }
+  if (!any) {                                                    // (the same in all CTAs of the cluster)
+    if (rank == 0 && tid == 0) { loss[row_at] = 0.f; stats[row_at * 2] = stats[row_at * 2 + 1] = make_float4(0.f, 0.f, 0.f, 0.f); }
     return;
   }
-  const float inv_t = 1.f / temp;
-  const T* x = logits + row * ld;
-  float m = -INFINITY;
-  for (int j = tid; j < V; j += TS_THREADS) m = fmaxf(m, to_f(x[j]));
-  m = rte::block_max(m, red);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float s = 0.f, so = 0.f;
-  for (int j = tid; j < V; j += TS_THREADS) {
-    bool listed = false;
-    if (tail) for (int i = 0; i < k; ++i) listed |= id[i] == j;
-    const float e = expf((to_f(x[j]) - ref) * inv_t);
-    s += e;
-    if (!listed) so += e;
-  }
-  s = rte::block_sum(s, red);
-  so = rte::block_sum(so, red);
-  if (tid == 0) {
-    double M = 0, L = 0, r = 0;
-    const double ln_s = log((double)s), shift = tail ? 0. : tmax + log(tsum);
-    for (int i = 0; i < k; ++i) {
-      if (id[i] < 0) continue;
-      const double lq = teacher[row * k + i] - shift, q = exp(lq);
-      M += q;
-      if (q != 0) L += q * (lq - (s == 0.f ? -INFINITY : (double)((to_f(x[id[i]]) - ref) * inv_t) - ln_s));
+  const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
+  Sums a = stream<T, NT, U, false, TAIL>(row, begin, end, c, 0, nullptr, id, k, bits);
+  a = block_sums<NT>(a, red);
+  if (C > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) mine = a;
+    cluster.sync();
+    a = no_sums();
+    for (int r = 0; r < C; ++r) {
+      Sums b = *cluster.map_shared_rank(&mine, r);
+      const float R = fmaxf(a.R, b.R);
+      move_to(a, R);
+      move_to(b, R);
+      a.top = fmaxf(a.top, b.top);
+      a.s += b.s;
     }
-    if (tail && so > 0.f) r = fmax(0., 1 - M);
-    if (r > 0) L += r * (log(r) - (log((double)so) - ln_s));
-    M += r;
-    loss[row] = float(L * temp * temp);
-    stats[row * 2] = make_float4(ref, (float)ln_s, float(M - (r > 0 ? r * (double)s / so : 0.)), s == 0.f ? 0.f : (float)M);
-    stats[row * 2 + 1] = make_float4((float)(tail ? 0. : tmax), (float)(tail ? 0. : log(tsum)), 0.f, 0.f);
+    if (careful(a)) {
+      const Sums b = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
+      cluster.sync();
+      if (tid == 0) mine = b;
+      cluster.sync();
+      a = b;
+      a.s = 0.f;
+      for (int r = 0; r < C; ++r) a.s += cluster.map_shared_rank(&mine, r)->s;
+    }
+    cluster.sync();                                              // (the others leave)
+    if (rank != 0) return;
+  } else if (careful(a)) {
+    a = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
   }
+  // in 64 bits from here: a few values per row, whose small differences are the loss
+  const double inv_t = 1. / temp;
+  const RowSum others(a, c);
+  double top = others.top, ln_s = others.ln_s, ln_out = 0;       // the row's; ln of the others' share of it
+  if (TAIL) {
+    float m = -INFINITY;
+    for (int i = tid; i < k; i += NT) if (id[i] >= 0) m = fmaxf(m, listed[i]);
+    top = block_max_float<NT>(fmaxf(m, a.top), red_f);
+    double s = 0;
+    if (top != -INFINITY)
+      for (int i = tid; i < k; i += NT) {
+        bool again = id[i] < 0;                                  // a token that an earlier slot names too counts once
+        for (int j = 0; j < i; ++j) again |= id[j] == id[i];
+        if (!again) s += exp((listed[i] - top) * inv_t);
+      }
+    s = block_sum_double<NT>(s, red_d);
+    const double ln_others = (others.top - top) * inv_t + others.ln_s;         // -inf: nothing outside the list
+    if (a.s != 0.f) s += exp(ln_others);
+    ln_s = log(s);
+    ln_out = ln_others - ln_s;
+  }
+  const bool none = top == -INFINITY && !(ln_s != ln_s);         // nothing but -inf
+  double shift = 0;
+  if (!TAIL) {
+    const float m = block_max_float<NT>(tmax, red_f);
+    double s = 0;
+    for (int i = tid; i < k; i += NT) if (id[i] >= 0) s += exp((double)t[i] - m);
+    s = block_sum_double<NT>(s, red_d);
+    tmax = m;
+    shift = log(s);
+  }
+  double M = 0, L = 0;
+  for (int i = tid; i < k; i += NT) {
+    if (id[i] < 0) continue;
+    const double lq = TAIL ? (double)t[i] : (double)t[i] - tmax - shift, q = exp(lq);
+    M += q;
+    if (q != 0) L += q * (lq - (none ? -INFINITY : (listed[i] - top) * inv_t - ln_s));
+  }
+  M = block_sum_double<NT>(M, red_d);
+  L = block_sum_double<NT>(L, red_d);
+  if (tid != 0) return;
+  const double r = TAIL && a.s > 0.f && !none ? fmax(0., 1 - M) : 0.;
+  if (r > 0) L += r * (log(r) - ln_out);
+  M += r;
+  loss[row_at] = float(L * temp * temp);
+  // log2 of the sum relative to the rounded reference that backward forms again
+  const Exponent ex((float)top, c);
+  const double l2 = ln_s * LOG2E + (ex.far ? 0. : top * c - ex.R);
+  stats[row_at * 2] = make_float4((float)top, (float)l2, float(M - (r > 0 ? r * exp(-ln_out) : 0.)), none ? 0.f : (float)M);
+  stats[row_at * 2 + 1] = make_float4(TAIL ? 0.f : tmax, (float)shift, 0.f, 0.f);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(TS_THREADS)
-distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float temp,
-                        const float4* __restrict__ stats, const float* __restrict__ dloss, T* __restrict__ dlogits, int V) {
+// ---------------------------------------------------------------- backward
+// A CTA per NT * U pieces of a row: p from the row's saved maximum and sum, the same for all columns; then the listed columns again.
+template <typename T, int NT, int U>
+struct Slice {
+  Row<T> row, out;
+  int first, end;                                                // pieces
+  __device__ __forceinline__ Slice(const T* x, T* dx, int V, int part) : row(x, V), out(dx, V), first(part * NT * U + threadIdx.x), end(row.pieces) {}
+  __device__ __forceinline__ bool holds(long long column, int part) const {
+    const long long v = (column + row.off) / Vec<T>::N - (long long)part * NT * U;
+    return column >= 0 && column < row.V && v >= 0 && v < NT * U;
+  }
+  __device__ __forceinline__ void store(int v, const float (&y)[Vec<T>::N]) const {
+    T* dx = const_cast<T*>(out.x);
+    const int c = row.column(v);
+    if (row.whole(v) && row.off == out.off) { *reinterpret_cast<uint4*>(dx + c) = Vec<T>::pack(y); return; }
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) if (c + i >= 0 && c + i < row.V) dx[c + i] = Vec<T>::from_f(y[i]);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) if (first + u * NT < end) raw[u] = row.load(first + u * NT);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (first + u * NT >= end) break;
+      float x[Vec<T>::N];
+      Vec<T>::unpack(raw[u], x);
+#pragma unroll
+      for (int i = 0; i < Vec<T>::N; ++i) x[i] = f(x[i]);
+      store(first + u * NT, x);
+    }
+  }
+  __device__ __forceinline__ void zero() const {
+    const float y[Vec<T>::N] = {};
+    for (int u = 0; u < U; ++u) if (first + u * NT < end) store(first + u * NT, y);
+  }
+};
+
+template <typename T, int NT, int U>
+__global__ void __launch_bounds__(NT)
+token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, float c, float inv_t, int k, const int64_t* __restrict__ top_ids,
+                          const float2* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ g_lp, const float* __restrict__ g_h,
+                          const float* __restrict__ g_top, T* __restrict__ dlogits, int V, int parts) {
   rte::after_previous_grid();
-  const long long row = blockIdx.x;
-  const float4 a = stats[row * 2], b = stats[row * 2 + 1];
-  T* dx = dlogits + row * V;
-  if (a.w == 0.f) {
-    for (int j = threadIdx.x; j < V; j += TS_THREADS) dx[j] = from_f<T>(0.f);
-    return;
+  __shared__ float red[NT / 32 > 0 ? NT / 32 : 1];
+  __shared__ int on_list;
+  const long long row_at = blockIdx.x / parts, tok = tokens[row_at];
+  const int part = blockIdx.x % parts, tid = threadIdx.x;
+  const float2 st = stats[row_at];
+  const Slice<T, NT, U> slice(logits + row_at * ld, dlogits + row_at * V, V, part);
+  if (tok < 0 || tok >= V || st.y == -INFINITY) return slice.zero();
+  const float g = g_lp ? g_lp[row_at] : 0.f, gh = g_h ? g_h[row_at] : 0.f;
+  float all = g;
+  if (!g_top) k = 0;
+  if (k > 0) {
+    float s = 0.f;
+    for (int i = tid; i < k; i += NT) s += g_top[row_at * k + i];
+    s = rte::warp_sum(s);
+    if (tid == 0) on_list = 0;
+    if (NT > 32) {
+      if ((tid & 31) == 0) red[tid >> 5] = s;
+      __syncthreads();
+      s = 0.f;
+      for (int w = 0; w < NT / 32; ++w) s += red[w];
+    } else {
+      __syncwarp();
+    }
+    all += s;
   }
-  const T* x = logits + row * ld;
-  const float scale = dloss[row] * temp, inv_t = 1.f / temp;
-  for (int j = threadIdx.x; j < V; j += TS_THREADS) {
-    const float p = expf((to_f(x[j]) - a.x) * inv_t - a.y);
-    bool listed = false;
-    float q = 0.f;
-    for (int i = 0; i < k; ++i)
-      if (ids[row * k + i] == j) { listed = true; q += expf(teacher[row * k + i] - b.x - b.y); }
-    dx[j] = from_f<T>(scale * (listed ? a.w * p - q : a.z * p));
+  // dx = -p (all + gh (ln p + H)) / T
+  const Exponent ex(st.x, c);
+  const float a = -(all + gh * entropy[row_at]) * inv_t, b = -gh * LN2 * inv_t;
+  const auto base = [&](float x) {
+    const float l = ex(x) - st.y;
+    return exp2_fast(l) * fmaf(b, weighted(l), a);
+  };
+  slice.each(base);
+  __syncthreads();
+  for (int i = tid; i < k; i += NT) {
+    const long long j = top_ids[row_at * k + i];
+    if (!slice.holds(j, part)) continue;
+    const bool target = j == tok;
+    if (target) on_list = 1;
+    dlogits[row_at * V + j] = Vec<T>::from_f(base(slice.row.at((int)j)) + (g_top[row_at * k + i] + (target ? g : 0.f)) * inv_t);
+  }
+  if (k > 0) __syncthreads();
+  if (tid == 0 && g_lp && slice.holds(tok, part) && !(k > 0 && on_list)) dlogits[row_at * V + tok] = Vec<T>::from_f(base(slice.row.at((int)tok)) + g * inv_t);
+}
+
+template <typename T, int NT, int U>
+__global__ void __launch_bounds__(NT)
+distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, float temp,
+                        const float4* __restrict__ stats, const float* __restrict__ dloss, T* __restrict__ dlogits, int V, int parts) {
+  rte::after_previous_grid();
+  __shared__ int id[TS_MAX_LIST];
+  __shared__ float q[TS_MAX_LIST];
+  const long long row_at = blockIdx.x / parts;
+  const int part = blockIdx.x % parts, tid = threadIdx.x;
+  const float4 st = stats[row_at * 2], list = stats[row_at * 2 + 1];
+  const Slice<T, NT, U> slice(logits + row_at * ld, dlogits + row_at * V, V, part);
+  if (st.w == 0.f) return slice.zero();
+  for (int i = tid; i < k; i += NT) {
+    const long long j = ids[row_at * k + i];
+    id[i] = slice.holds(j, part) ? (int)j : -1;
+    if (id[i] >= 0) q[i] = expf(teacher[row_at * k + i] - list.x - list.y);
+  }
+  const Exponent ex(st.x, c);
+  const float scale = dloss[row_at] * temp, outside = scale * st.z, inside = scale * st.w;
+  slice.each([&](float x) { return exp2_fast(ex(x) - st.y) * outside; });
+  __syncthreads();
+  for (int i = tid; i < k; i += NT) {
+    if (id[i] < 0) continue;
+    bool again = false;                                          // a token named by several slots: the first of them writes
+    float sum = 0.f;
+    for (int j = 0; j < k; ++j)
+      if (id[j] == id[i]) { again |= j < i; sum += q[j]; }
+    if (!again) dlogits[row_at * V + id[i]] = Vec<T>::from_f(exp2_fast(ex(slice.row.at(id[i])) - st.y) * inside - scale * sum);
   }
 }
 
-bool temperature_ok(float t) { return t > 0.f && t <= 1e30f && 1.f / t <= 1e30f; }
-bool type_ok(int type) { return type == RTE_TYPE_BF16 || type == RTE_TYPE_F16 || type == RTE_TYPE_F32; }
+// ---------------------------------------------------------------- launches
+template <typename K, typename... A>
+void launch_cluster(K kernel, long long ctas, int nt, size_t smem, int C, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(nt);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = C > 1 ? 2 : 1;
+  (void)cudaLaunchKernelEx(&cfg, kernel, args...);               // (an error stays pending for RTE_LAUNCH_CHECK)
+}
+
+// CTAs per row: as many (up to 8) as bring two CTAs to every SM, with a tile of pieces each.
+int cluster_of(long long rows, int pieces, int tile) {
+  int C = 1;
+  while (C < 8 && rows * C < 2 * 148 && pieces > C * tile) C *= 2;
+  return C;
+}
+// The most pieces a row of V columns has: one more where rows do not all start on 16 bytes.
+int pieces_of(const void* x, int type, long long ld, int V) {
+  const int size = type == RTE_TYPE_F32 ? 4 : 2, n = 16 / size;
+  const bool even = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * size % 16 == 0;
+  return int(((long long)V + (even ? n - 1 : 2 * n - 2)) / n);
+}
+
+// A row of at most one tile of 32 or 128 threads is one CTA of them; longer ones are walked by 256.
+#define BY_SIZE(T, pieces, CALL)          \
+  do {                                    \
+    if (pieces <= 128) CALL(T, 32, 4);    \
+    else if (pieces <= 512) CALL(T, 128, 4); \
+    else CALL(T, 256, 4);                 \
+  } while (0)
+#define BY_TYPE_AND_SIZE(type, pieces, CALL)                      \
+  do {                                                            \
+    if (type == RTE_TYPE_BF16) BY_SIZE(__nv_bfloat16, pieces, CALL); \
+    else if (type == RTE_TYPE_F16) BY_SIZE(__half, pieces, CALL); \
+    else BY_SIZE(float, pieces, CALL);                            \
+  } while (0)
+
+bool temperature_ok(float t) { return t >= 1e-30f && t <= 1e30f; }
+bool rows_ok(const void* x, int type, int64_t ldl, int64_t rows, int64_t V) {
+  return x && (type == RTE_TYPE_BF16 || type == RTE_TYPE_F16 || type == RTE_TYPE_F32) && rows > 0 && V > 0 && V <= TS_MAX_V && ldl >= 0;
+}
+bool on_element(const void* x, int type) { return reinterpret_cast<uintptr_t>(x) % (type == RTE_TYPE_F32 ? 4 : 2) == 0; }
+float log2_scale(float temperature) { return (float)(LOG2E / temperature); }
 
 }  // namespace
 
 #define ST(s) static_cast<cudaStream_t>(s)
-#define BY_TYPE(type, CALL)                             \
-  do {                                                  \
-    if (type == RTE_TYPE_BF16) CALL(__nv_bfloat16);     \
-    else if (type == RTE_TYPE_F16) CALL(__half);        \
-    else CALL(float);                                   \
-  } while (0)
 
 extern "C" int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t ldl, const int64_t* tokens, int64_t ignore_index, float temperature, int32_t top_k,
                                       float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, float* row_stats, int32_t rows, int32_t V, int32_t* status,
                                       rte_stream_t stream) {
-  RTE_CHECK_ARG(logits && tokens && logprob && entropy && row_stats && type_ok(type) && rows > 0 && V > 0 && ldl >= 0 && temperature_ok(temperature));
+  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && tokens && logprob && entropy && row_stats && temperature_ok(temperature));
   RTE_CHECK_ARG(top_k >= 0 && top_k <= V && top_k <= TS_MAX_LIST && (top_k == 0 || (top_logprobs && top_ids)));
-#define CALL(T)                                                                                                                                                     \
-  rte::launch(token_logprobs_kernel<T>, rows, TS_THREADS, 0, ST(stream), static_cast<const T*>(logits), ldl, tokens, ignore_index, 1.f / temperature, top_k, logprob, \
-              entropy, top_logprobs, top_ids, reinterpret_cast<float2*>(row_stats), V, status)
-  BY_TYPE(type, CALL);
+  if (!on_element(logits, type) || reinterpret_cast<uintptr_t>(row_stats) % 8) return RTE_ERR_ALIGNMENT;
+  const int pieces = pieces_of(logits, type, ldl, V);
+#define CALL(T, NT, U)                                                                                                                                       \
+  do {                                                                                                                                                       \
+    const int C = cluster_of(rows, pieces, NT * U);                                                                                                          \
+    launch_cluster(token_logprobs_kernel<T, NT, U>, (long long)rows * C, NT, top_k > 0 ? sizeof(TopK<NT, U>) : 0, C, ST(stream), static_cast<const T*>(logits), \
+                   (long long)ldl, tokens, (long long)ignore_index, log2_scale(temperature), 1. / temperature, (int)top_k, logprob, entropy, top_logprobs,    \
+                   top_ids, reinterpret_cast<float2*>(row_stats), (int)V, C, status);                                                                        \
+  } while (0)
+  BY_TYPE_AND_SIZE(type, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -238,12 +823,19 @@ extern "C" int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t 
 extern "C" int rte_token_logprobs_bwd(const void* logits, int32_t type, int64_t ldl, const int64_t* tokens, float temperature, int32_t top_k, const int64_t* top_ids,
                                       const float* row_stats, const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_top, void* dlogits,
                                       int32_t rows, int32_t V, rte_stream_t stream) {
-  RTE_CHECK_ARG(logits && tokens && entropy && row_stats && dlogits && type_ok(type) && rows > 0 && V > 0 && ldl >= 0 && temperature_ok(temperature));
+  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && tokens && entropy && row_stats && dlogits && temperature_ok(temperature));
   RTE_CHECK_ARG(top_k >= 0 && top_k <= V && top_k <= TS_MAX_LIST && (!g_top || top_k == 0 || top_ids));
-#define CALL(T)                                                                                                                                                      \
-  rte::launch(token_logprobs_bwd_kernel<T>, rows, TS_THREADS, 0, ST(stream), static_cast<const T*>(logits), ldl, tokens, 1.f / temperature, top_k, top_ids,           \
-              reinterpret_cast<const float2*>(row_stats), entropy, g_logprob, g_entropy, g_top, static_cast<T*>(dlogits), V)
-  BY_TYPE(type, CALL);
+  if (!on_element(logits, type) || !on_element(dlogits, type) || reinterpret_cast<uintptr_t>(row_stats) % 8) return RTE_ERR_ALIGNMENT;
+  const int pieces = pieces_of(logits, type, ldl, V);
+#define CALL(T, NT, U)                                                                                                                                        \
+  do {                                                                                                                                                        \
+    const int parts = rte::ceil_div(pieces, NT * U);                                                                                                          \
+    if ((long long)rows * parts > 0x7fffffff) return RTE_ERR_UNSUPPORTED;                                                                                      \
+    rte::launch(token_logprobs_bwd_kernel<T, NT, U>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, tokens, log2_scale(temperature),     \
+                1.f / temperature, top_k, top_ids, reinterpret_cast<const float2*>(row_stats), entropy, g_logprob, g_entropy, g_top, static_cast<T*>(dlogits), V, \
+                parts);                                                                                                                                       \
+  } while (0)
+  BY_TYPE_AND_SIZE(type, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -251,13 +843,18 @@ extern "C" int rte_token_logprobs_bwd(const void* logits, int32_t type, int64_t 
 
 extern "C" int rte_distill_topk_fwd(const void* logits, int32_t type, int64_t ldl, const float* teacher, const int64_t* ids, int32_t k, float temperature, int32_t tail,
                                     float* loss, float* row_stats, int32_t rows, int32_t V, int32_t* status, rte_stream_t stream) {
-  RTE_CHECK_ARG(logits && teacher && ids && loss && row_stats && type_ok(type) && rows > 0 && V > 0 && ldl >= 0 && temperature_ok(temperature));
+  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && teacher && ids && loss && row_stats && temperature_ok(temperature));
   RTE_CHECK_ARG(k > 0 && k <= TS_MAX_LIST);
-  if (reinterpret_cast<uintptr_t>(row_stats) & 15) return RTE_ERR_ALIGNMENT;
-#define CALL(T)                                                                                                                                                     \
-  rte::launch(distill_topk_kernel<T>, rows, TS_THREADS, 0, ST(stream), static_cast<const T*>(logits), ldl, teacher, ids, k, temperature, tail, loss,                  \
-              reinterpret_cast<float4*>(row_stats), V, status)
-  BY_TYPE(type, CALL);
+  if (!on_element(logits, type) || reinterpret_cast<uintptr_t>(row_stats) % 16) return RTE_ERR_ALIGNMENT;
+  const int pieces = pieces_of(logits, type, ldl, V);
+#define CALL(T, NT, U)                                                                                                                                         \
+  do {                                                                                                                                                         \
+    const int C = cluster_of(rows, pieces, NT * U);                                                                                                            \
+    launch_cluster(tail ? distill_topk_kernel<T, NT, U, true> : distill_topk_kernel<T, NT, U, false>, (long long)rows * C, NT, 0, C, ST(stream),               \
+                   static_cast<const T*>(logits), (long long)ldl, teacher, ids, (int)k, log2_scale(temperature), (double)temperature, loss,                    \
+                   reinterpret_cast<float4*>(row_stats), (int)V, C, status);                                                                                   \
+  } while (0)
+  BY_TYPE_AND_SIZE(type, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -265,13 +862,18 @@ extern "C" int rte_distill_topk_fwd(const void* logits, int32_t type, int64_t ld
 
 extern "C" int rte_distill_topk_bwd(const void* logits, int32_t type, int64_t ldl, const float* teacher, const int64_t* ids, int32_t k, float temperature,
                                     const float* row_stats, const float* dloss, void* dlogits, int32_t rows, int32_t V, rte_stream_t stream) {
-  RTE_CHECK_ARG(logits && teacher && ids && row_stats && dloss && dlogits && type_ok(type) && rows > 0 && V > 0 && ldl >= 0 && temperature_ok(temperature));
+  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && teacher && ids && row_stats && dloss && dlogits && temperature_ok(temperature));
   RTE_CHECK_ARG(k > 0 && k <= TS_MAX_LIST);
-  if (reinterpret_cast<uintptr_t>(row_stats) & 15) return RTE_ERR_ALIGNMENT;
-#define CALL(T)                                                                                                                                                 \
-  rte::launch(distill_topk_bwd_kernel<T>, rows, TS_THREADS, 0, ST(stream), static_cast<const T*>(logits), ldl, teacher, ids, k, temperature,                      \
-              reinterpret_cast<const float4*>(row_stats), dloss, static_cast<T*>(dlogits), V)
-  BY_TYPE(type, CALL);
+  if (!on_element(logits, type) || !on_element(dlogits, type) || reinterpret_cast<uintptr_t>(row_stats) % 16) return RTE_ERR_ALIGNMENT;
+  const int pieces = pieces_of(logits, type, ldl, V);
+#define CALL(T, NT, U)                                                                                                                                       \
+  do {                                                                                                                                                       \
+    const int parts = rte::ceil_div(pieces, NT * U);                                                                                                         \
+    if ((long long)rows * parts > 0x7fffffff) return RTE_ERR_UNSUPPORTED;                                                                                     \
+    rte::launch(distill_topk_bwd_kernel<T, NT, U>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, teacher, ids, k, log2_scale(temperature), \
+                temperature, reinterpret_cast<const float4*>(row_stats), dloss, static_cast<T*>(dlogits), V, parts);                                          \
+  } while (0)
+  BY_TYPE_AND_SIZE(type, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;

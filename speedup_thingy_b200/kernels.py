@@ -208,7 +208,7 @@ class TokenLogprobs(NamedTuple):
 def _check_scores(name: str, logits, temperature, *others) -> None:
     if logits.dtype not in _LOGIT_TYPES:
         raise ValueError(f"{name}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
-    if logits.ndim == 0 or not 1 <= logits.shape[-1] < 2 ** 31:
+    if logits.ndim == 0 or not 1 <= logits.shape[-1] < 2 ** 31 - 256:
         raise ValueError(f"{name}: logits [..., V] with at least one column, got {tuple(logits.shape)}")
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"{name}: the temperature must be positive and finite, got {temperature}")
