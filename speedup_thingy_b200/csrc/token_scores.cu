@@ -31,8 +31,14 @@ __device__ __forceinline__ float exp2_fast(float t) {            // two units in
   return r;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {     // NaN where either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ---------------------------------------------------------------- 16 bytes of a row
-template <typename T> struct Vec;              // N values; pairs() takes them two at a time
+template <typename T> struct Vec;              // N values; max: NaN where one of them is
 template <> struct Vec<float> {
   static constexpr int N = 4;
   static constexpr uint32_t NONE = 0xff800000u;                  // -inf
@@ -40,7 +46,7 @@ template <> struct Vec<float> {
     x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
   }
   static __device__ __forceinline__ float max(const uint4& r) {
-    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)), max_nan(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
@@ -58,8 +64,8 @@ template <> struct Vec<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float max(const uint4& r) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
     return make_uint4(rte::pack_bf16x2(x[0], x[1]), rte::pack_bf16x2(x[2], x[3]), rte::pack_bf16x2(x[4], x[5]), rte::pack_bf16x2(x[6], x[7]));
@@ -77,8 +83,8 @@ template <> struct Vec<__half> {
   }
   static __device__ __forceinline__ float max(const uint4& r) {
     const __half2* h = reinterpret_cast<const __half2*>(&r);
-    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
     uint4 r;
@@ -179,21 +185,27 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
   return u == 0xfffffffeu ? __uint_as_float(0x7fffffffu) : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-// Candidates are what reaches a bound that at least k logits reach: the first tile's bound is the k-th largest of its 16-byte pieces'
-// maxima, later ones are the k-th largest candidate.  k + a few candidates pass in a tile of unordered logits.
-template <int NT, int U>
-struct TopK {
-  static constexpr int CAP = 2048;                       // candidates kept (the largest list and a warp's tile of pieces fit more than once)
-  static constexpr int PIECES = NT * U;
-  unsigned long long cand[CAP];
-  unsigned long long list[TS_MAX_LIST];
-  uint32_t piece_max[PIECES];
-  unsigned long long bound;
-  int count, held, listed;
+// The k largest logits lie in the k pieces (16 bytes of the row) whose own largest logits come first, equal ones by the lower piece: every
+// other piece holds only what k logits come before.  So the search goes over pieces, an eighth or a quarter of the columns: those that
+// reach a bound are noted, the bound is the k-th of what has been seen (the first one the k-th of the threads' largest, so that a
+// few more than k pieces of a tile pass), and only in the end the columns of the last k pieces, and a few more, are ordered.
+__host__ __device__ constexpr int slack_of(int k) { return k / 8 + 4; }
+struct TopK {                                            // in shared memory, sized by k: `shared_bytes`
+  struct Head { unsigned long long bound; int count, keep; };
+  Head& h;
+  unsigned long long *kept, *piece;                      // [k + slack], [cap]: value | ~piece; in the end value | ~column
+  uint32_t* top;                                         // [threads]
+  int k, cap;
+  // a tile's pieces behind twice what is kept; all columns of the pieces kept, which is also what 8 slices keep
+  static __host__ __device__ int cap_of(int k, int tile) { return max(tile + 2 * (k + slack_of(k)), 8 * (k + slack_of(k))); }
+  static size_t shared_bytes(int k, int nt, int u) { return sizeof(Head) + 8 * ((size_t)k + slack_of(k) + cap_of(k, nt * u)) + 4 * (size_t)nt; }
+  __device__ __forceinline__ TopK(unsigned char* at, int k_, int tile)
+      : h(*reinterpret_cast<Head*>(at)), kept(reinterpret_cast<unsigned long long*>(at + sizeof(Head))), piece(kept + k_ + slack_of(k_)),
+        top(reinterpret_cast<uint32_t*>(piece + cap_of(k_, tile))), k(k_), cap(cap_of(k_, tile)) {}
 };
 
 // The largest bound that at least k (at most k + slack, unless equal keys forbid) of n keys reach; one warp, keys `step` words apart.
-__device__ uint32_t warp_bound(const uint32_t* keys, int n, int step, int k, int slack, int* reach) {
+__device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int step, int k, int slack, int* reach) {
   const int lane = threadIdx.x & 31;
   uint32_t lo = 0xffffffffu, hi = 0;
   for (int i = lane; i < n; i += 32) { lo = min(lo, keys[i * step]); hi = max(hi, keys[i * step]); }
@@ -203,6 +215,7 @@ __device__ uint32_t warp_bound(const uint32_t* keys, int n, int step, int k, int
   while (hi - lo > 1 && at_lo > k + slack) {
     const uint32_t mid = lo + (hi - lo) / 2;
     int c = 0;
+#pragma unroll 4
     for (int i = lane; i < n; i += 32) c += keys[i * step] >= mid;
     c = __reduce_add_sync(0xffffffffu, c);
     if (c >= k) { lo = mid; at_lo = c; } else hi = mid;
@@ -211,109 +224,107 @@ __device__ uint32_t warp_bound(const uint32_t* keys, int n, int step, int k, int
   return lo;
 }
 
-// The k-th largest candidate (0: there are no more than k), by one warp.
-__device__ unsigned long long warp_kth(const unsigned long long* cand, int n, int k) {
-  if (n <= k) return 0;
+// A bound that at least k and at most k + slack of n distinct keys reach (0: all), by one warp.
+__device__ unsigned long long warp_bound64(const unsigned long long* keys, int n, int k, int slack) {
+  if (n <= k + slack) return 0;
   const int lane = threadIdx.x & 31;
   int reach;
-  const uint32_t value = warp_bound(reinterpret_cast<const uint32_t*>(cand) + 1, n, 2, k, 0, &reach);
-  if (reach == k) return (unsigned long long)value << 32;
-  int above = 0;                                         // equal values at the end of the list: the lowest columns
-  for (int i = lane; i < n; i += 32) above += uint32_t(cand[i] >> 32) > value;
+  const uint32_t value = warp_bound(reinterpret_cast<const uint32_t*>(keys) + 1, n, 2, k, slack, &reach);
+  if (reach <= k + slack) return (unsigned long long)value << 32;
+  int above = 0;                                         // many equal values at the end: the lowest of their columns
+  for (int i = lane; i < n; i += 32) above += uint32_t(keys[i] >> 32) > value;
   const int want = k - __reduce_add_sync(0xffffffffu, above);
-  uint32_t lo = 0, hi = 0xffffffffu;                     // (column 0 has the key ~0: reached by `lo` alone)
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
+  unsigned long long lo = 0, hi = 1ull << 32;
+  int at_lo = reach - (k - want);
+  while (hi - lo > 1 && at_lo > want + slack) {
+    const unsigned long long mid = lo + (hi - lo) / 2;
     int c = 0;
-    for (int i = lane; i < n; i += 32) c += uint32_t(cand[i] >> 32) == value && uint32_t(cand[i]) >= mid;
-    if (__reduce_add_sync(0xffffffffu, c) >= want) lo = mid; else hi = mid;
+    for (int i = lane; i < n; i += 32) c += uint32_t(keys[i] >> 32) == value && uint32_t(keys[i]) >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= want) { lo = mid; at_lo = c; } else hi = mid;
   }
-  int c = 0;
-  for (int i = lane; i < n; i += 32) c += uint32_t(cand[i] >> 32) == value && uint32_t(cand[i]) >= hi;
-  if (__reduce_add_sync(0xffffffffu, c) >= want) lo = hi;
   return (unsigned long long)value << 32 | lo;
 }
 
-// list = the k largest of the first n candidates (all of them if there are no more), in any order; `listed` of them; `bound`: the last.
-template <typename S, int NT>
-__device__ void select(S& S_, int n, int k) {
+// kept = those of the first `count` keys that reach a bound which k to k + slack of them reach (all, if there are no more); keep: how many.
+template <int NT>
+__device__ __forceinline__ void thin(TopK& S) {
   __syncthreads();
+  const int n = S.h.count;
   if (threadIdx.x < 32) {
-    const unsigned long long b = warp_kth(S_.cand, n, k);
-    if (threadIdx.x == 0) { S_.bound = b; S_.listed = 0; }
+    const unsigned long long b = warp_bound64(S.piece, n, S.k, slack_of(S.k));
+    if (threadIdx.x == 0) { S.h.bound = b > S.h.bound ? b : S.h.bound; S.h.keep = 0; }
   }
   __syncthreads();
-  const unsigned long long b = S_.bound;
-  for (int i = threadIdx.x; i < n; i += NT)
-    if (S_.cand[i] >= b) S_.list[atomicAdd(&S_.listed, 1)] = S_.cand[i];
+  const unsigned long long b = S.h.bound;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const unsigned long long key = S.piece[i];
+    if (key >= b) S.kept[atomicAdd(&S.h.keep, 1)] = key;
+  }
   __syncthreads();
 }
 
-// Adds a tile's pieces (raw[u]: piece first + u * NT of the row) to the candidates.  `looked`: this thread's pieces may hold a NaN.
-template <typename T, int NT, int U>
-__device__ __forceinline__ void collect(TopK<NT, U>& S, const Row<T>& row, const uint4 (&raw)[U], const float (&top)[U], int first, int end, int k, bool start, bool looked) {
-  constexpr int N = Vec<T>::N;
+// Notes a tile's pieces (top[u]: the largest of piece first + u * NT, below `end`; all: of this thread's) that reach the bound.  Whether
+// this thread found no room for another tile behind its own.
+template <int NT, int U>
+__device__ __forceinline__ bool note(TopK& S, const float (&top)[U], float all, int first, int end, bool start) {
   const int tid = threadIdx.x;
   if (start) {
-    int have = 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = first + u * NT < end;
-      S.piece_max[u * NT + tid] = in ? value_key(top[u]) : 0;
-      have += in;
-    }
-    if (tid == 0) { S.count = 0; S.held = TopK<NT, U>::CAP; }
+    const int n = min(end - (first - tid), NT);          // threads with a piece
+    S.top[tid] = value_key(all);
+    if (tid == 0) S.h.count = 0;
     __syncthreads();
     if (tid < 32) {
-      const int n = min(max(end - (first - tid), 0), NT * U);          // the pieces of the tile, one after the other
       int reach;
-      const uint32_t b = n > k ? warp_bound(S.piece_max, n, 1, k, k / 8, &reach) : 0;
-      if (tid == 0) S.bound = (unsigned long long)b << 32;
+      const uint32_t b = n > S.k ? warp_bound(S.top, n, 1, S.k, S.k / 8, &reach) : 0;
+      if (tid == 0) S.h.bound = (unsigned long long)b << 32;
     }
     __syncthreads();
   }
-  uint32_t todo = 0;
-  {
-    const uint32_t bound = uint32_t(S.bound >> 32);
+  const unsigned long long bound = S.h.bound;
+  const float least = key_value(bound);                  // (NaN: no bound, or NaN is)
+  int last = -1;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (first + u * NT < end && (looked || value_key(top[u]) >= bound)) todo |= 1u << u;
+  for (int u = 0; u < U; ++u) {
+    if (first + u * NT >= end || top[u] < least) continue;
+    const unsigned long long key = order_key(top[u], first + u * NT);
+    if (key >= bound) S.piece[last = atomicAdd(&S.h.count, 1)] = key;
   }
-  while (true) {
-    const unsigned long long bound = S.bound;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!(todo >> u & 1)) continue;
-      float x[N];
-      Vec<T>::unpack(raw[u], x);
-      const int c = row.column(first + u * NT);
-      uint32_t pass = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (c + i >= 0 && c + i < row.V && order_key(x[i], c + i) >= bound) pass |= 1u << i;
-      const int n = __popc(pass);
-      if (n == 0) { todo &= ~(1u << u); continue; }
-      int at = atomicAdd(&S.count, n);
-      if (at + n > TopK<NT, U>::CAP) { atomicMin(&S.held, at); continue; }
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (pass >> i & 1) S.cand[at++] = order_key(x[i], c + i);
-      todo &= ~(1u << u);
-    }
-    if (!__syncthreads_or(todo)) break;
-    // full: only the k largest stay, and the rest of the tile has to reach the last of them
-    select<TopK<NT, U>, NT>(S, S.held, k);
-    const int n = S.listed;
-    for (int i = tid; i < n; i += NT) S.cand[i] = S.list[i];
-    if (tid == 0) { S.count = n; S.held = TopK<NT, U>::CAP; }
-    __syncthreads();
+  return last >= S.cap - NT * U;
+}
+// Behind a tile that another one follows: room for all of its pieces.
+template <int NT>
+__device__ __forceinline__ void make_room(TopK& S, bool full) {
+  if (!__syncthreads_or(full)) return;                   // (the count itself may grow while others still look)
+  thin<NT>(S);
+  const int n = S.h.keep;
+  for (int i = threadIdx.x; i < n; i += NT) S.piece[i] = S.kept[i];
+  if (threadIdx.x == 0) S.h.count = n;
+  __syncthreads();
+}
+// In the end: kept = columns among which the row's (the slice's) k largest logits are, `keep` of them, no more than k + slack.
+template <typename T, int NT>
+__device__ __forceinline__ void columns(TopK& S, const Row<T>& row) {
+  constexpr int N = Vec<T>::N;
+  thin<NT>(S);
+  const int pieces = S.h.keep;
+  const unsigned long long bound = S.h.bound & 0xffffffff00000000ull;     // (of k pieces' largest: k columns reach its value)
+  __syncthreads();
+  if (threadIdx.x == 0) { S.h.count = 0; S.h.bound = bound; }
+  __syncthreads();
+  for (int i = threadIdx.x; i < pieces * N; i += NT) {
+    const int c = row.column((int)~(uint32_t)S.kept[i / N]) + i % N;
+    if (c < 0 || c >= row.V) continue;
+    const unsigned long long key = order_key(row.at(c), c);
+    if (key >= bound) S.piece[atomicAdd(&S.h.count, 1)] = key;
   }
+  thin<NT>(S);
 }
 
 // ---------------------------------------------------------------- one pass over a row's pieces [begin, end)
 // OUTSIDE: the columns of `id` (-1: none) are left out; `bits`: a bit per column of a tile, in shared memory.
-template <typename T, int NT, int U, bool ENTROPY, bool OUTSIDE>
-__device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, float c, int k, TopK<NT, U>* top_k, const int* id, int ids, uint32_t* bits) {
+template <typename T, int NT, int U, bool ENTROPY, bool TOP, bool OUTSIDE>
+__device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, float c, TopK* top_k, const int* id, int ids, uint32_t* bits) {
   constexpr int N = Vec<T>::N, TILE = NT * U;
   const int tid = threadIdx.x;
   Sums a = no_sums();
@@ -348,7 +359,7 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
     }
     float top[U], all = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) { top[u] = Vec<T>::max(raw[u]); all = fmaxf(all, top[u]); }
+    for (int u = 0; u < U; ++u) { top[u] = Vec<T>::max(raw[u]); all = TOP ? max_nan(all, top[u]) : fmaxf(all, top[u]); }
     if (all > a.top) {
       a.top = all;
       const float R = fmaxf(a.R, all * c);
@@ -371,7 +382,10 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
     s[0] += s[1];
     a.s += s[0];
     if (ENTROPY) a.e += e[0] + e[1];
-    if (k > 0) collect<T, NT, U>(*top_k, row, raw, top, first, end, k, tile == begin, s[0] != s[0]);
+    if (TOP) {
+      const bool full = note<NT, U>(*top_k, top, all, first, end, tile == begin);
+      if (tile + TILE < end) make_room<NT>(*top_k, full);
+    }
   }
   return a;
 }
@@ -396,13 +410,13 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
 
 // ---------------------------------------------------------------- forward
 // A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.
-template <typename T, int NT, int U>
-__global__ void __launch_bounds__(NT)
+template <typename T, int NT, int U, bool TOP>
+__global__ void __launch_bounds__(NT, 1280 / NT > 20 ? 20 : 1280 / NT)
 token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, double inv_t, int k, float* __restrict__ logprob,
                       float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids, float2* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
   extern __shared__ __align__(16) unsigned char dyn[];
-  TopK<NT, U>* top = reinterpret_cast<TopK<NT, U>*>(dyn);       // (there is none where k = 0)
+  TopK top(dyn, k, NT * U);                                      // (there is none without TOP)
   __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
   __shared__ Sums mine;
   const long long row_at = blockIdx.x / C;
@@ -420,11 +434,11 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   float target = 0.f;
   if (rank == 0 && tid == 0) target = row.at((int)tok);
   const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
-  Sums a = stream<T, NT, U, true, false>(row, begin, end, c, k, top, nullptr, 0, nullptr);
+  Sums a = stream<T, NT, U, true, TOP, false>(row, begin, end, c, &top, nullptr, 0, nullptr);
   a = block_sums<NT>(a, red);
-  if (k > 0) {
-    if (begin < end) select<TopK<NT, U>, NT>(*top, top->count, k);
-    else if (tid == 0) top->listed = 0;
+  if (TOP) {
+    if (begin < end) columns<T, NT>(top, row);
+    else if (tid == 0) { top.h.keep = 0; top.h.bound = 0; }
   }
   if (C > 1) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -449,16 +463,17 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
       a.s = a.e = 0.f;
       for (int r = 0; r < C; ++r) { const Sums* o = cluster.map_shared_rank(&mine, r); a.s += o->s; a.e += o->e; }
     }
-    if (k > 0 && rank == 0) {
+    if (TOP && rank == 0) {
       int n = 0;
       for (int r = 0; r < C; ++r) {
-        const TopK<NT, U>* o = cluster.map_shared_rank(top, r);
-        const int m = o->listed;
-        for (int i = tid; i < m; i += NT) top->cand[n + i] = o->list[i];
+        const unsigned long long* kept = cluster.map_shared_rank(top.kept, r);
+        const int m = cluster.map_shared_rank(&top.h, r)->keep;
+        for (int i = tid; i < m; i += NT) top.piece[n + i] = kept[i];
         n += m;
       }
+      if (tid == 0) top.h.count = n;
       cluster.sync();                                            // (the others leave)
-      select<TopK<NT, U>, NT>(*top, n, k);
+      thin<NT>(top);
     } else {
       cluster.sync();
     }
@@ -474,10 +489,14 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
     entropy[row_at] = none ? 0.f : LN2 * (log2f(a.s) - a.e / a.s);
     stats[row_at] = make_float2(a.top, none ? -INFINITY : log2f(a.s));
   }
-  for (int i = tid; i < k; i += NT) {                            // the list's order: how many keys are larger
-    const unsigned long long key = top->list[i];
+  if (!TOP) return;
+  const int n = top.h.keep;
+  for (int i = tid; i < n; i += NT) {                            // the list's order: how many keys come before
+    const unsigned long long key = top.kept[i];
     int before = 0;
-    for (int j = 0; j < k; ++j) before += top->list[j] > key;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) before += top.kept[j] > key;
+    if (before >= k) continue;
     top_ids[row_at * k + before] = (int)~(uint32_t)key;
     top_lp[row_at * k + before] = none ? -INFINITY : (float)sum.logprob(key_value(key), inv_t);
   }
@@ -541,7 +560,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
     return;
   }
   const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
-  Sums a = stream<T, NT, U, false, TAIL>(row, begin, end, c, 0, nullptr, id, k, bits);
+  Sums a = stream<T, NT, U, false, false, TAIL>(row, begin, end, c, nullptr, id, k, bits);
   a = block_sums<NT>(a, red);
   if (C > 1) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -810,8 +829,9 @@ extern "C" int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t 
 #define CALL(T, NT, U)                                                                                                                                       \
   do {                                                                                                                                                       \
     const int C = cluster_of(rows, pieces, NT * U);                                                                                                          \
-    launch_cluster(token_logprobs_kernel<T, NT, U>, (long long)rows * C, NT, top_k > 0 ? sizeof(TopK<NT, U>) : 0, C, ST(stream), static_cast<const T*>(logits), \
-                   (long long)ldl, tokens, (long long)ignore_index, log2_scale(temperature), 1. / temperature, (int)top_k, logprob, entropy, top_logprobs,    \
+    launch_cluster(top_k > 0 ? token_logprobs_kernel<T, NT, U, true> : token_logprobs_kernel<T, NT, U, false>, (long long)rows * C, NT,                      \
+                   top_k > 0 ? TopK::shared_bytes(top_k, NT, U) : 0, C, ST(stream), static_cast<const T*>(logits), (long long)ldl,                                         \
+                   tokens, (long long)ignore_index, log2_scale(temperature), 1. / temperature, (int)top_k, logprob, entropy, top_logprobs,    \
                    top_ids, reinterpret_cast<float2*>(row_stats), (int)V, C, status);                                                                        \
   } while (0)
   BY_TYPE_AND_SIZE(type, pieces, CALL);
