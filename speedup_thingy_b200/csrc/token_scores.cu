@@ -19,6 +19,10 @@ namespace cg = cooperative_groups;
 
 namespace {
 
+#ifndef TS_MB32
+#define TS_MB32 24
+#define TS_MB128 10
+#endif
 constexpr int TS_MAX_LIST = RTE_TOKEN_LIST_MAX;
 constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
 constexpr float LN2 = 0.693147180559945309f;
@@ -40,6 +44,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {     // NaN where ei
 // ---------------------------------------------------------------- 16 bytes of a row
 template <typename T> struct Vec;              // N values; max: NaN where one of them is
 template <> struct Vec<float> {
+  static constexpr int SHIFT = 0;                       // low bits that a value's key does not use
   static constexpr int N = 4;
   static constexpr uint32_t NONE = 0xff800000u;                  // -inf
   static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[4]) {
@@ -55,6 +60,7 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ float from_f(float v) { return v; }
 };
 template <> struct Vec<__nv_bfloat16> {
+  static constexpr int SHIFT = 16;
   static constexpr int N = 8;
   static constexpr uint32_t NONE = 0xff80ff80u;
   static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[8]) {
@@ -74,6 +80,7 @@ template <> struct Vec<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 };
 template <> struct Vec<__half> {
+  static constexpr int SHIFT = 13;
   static constexpr int N = 8;
   static constexpr uint32_t NONE = 0xfc00fc00u;
   static __device__ __forceinline__ void unpack(const uint4& r, float (&x)[8]) {
@@ -189,136 +196,209 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
 // other piece holds only what k logits come before.  So the search goes over pieces, an eighth or a quarter of the columns: those that
 // reach a bound are noted, the bound is the k-th of what has been seen (the first one the k-th of the threads' largest, so that a
 // few more than k pieces of a tile pass), and only in the end the columns of the last k pieces, and a few more, are ordered.
-__host__ __device__ constexpr int slack_of(int k) { return k / 8 + 4; }
+__host__ __device__ constexpr int slack_of(int k) { return k / 2 + 16 + ((k + k / 2) & 1); }       // (k + slack is even)
 struct TopK {                                            // in shared memory, sized by k: `shared_bytes`
-  struct Head { unsigned long long bound; int count, keep; };
+  struct Head { unsigned long long bound; int count, keep, from, pad[3]; };
   Head& h;
-  unsigned long long *kept, *piece;                      // [k + slack], [cap]: value | ~piece; in the end value | ~column
+  unsigned long long *kept, *piece;                      // [k + slack], [cap]: value | ~piece; from piece + k + slack on, in the end: value | ~column
   uint32_t* top;                                         // [threads]
   int k, cap;
-  // a tile's pieces behind twice what is kept; all columns of the pieces kept, which is also what 8 slices keep
-  static __host__ __device__ int cap_of(int k, int tile) { return max(tile + 2 * (k + slack_of(k)), 8 * (k + slack_of(k))); }
-  static size_t shared_bytes(int k, int nt, int u) { return sizeof(Head) + 8 * ((size_t)k + slack_of(k) + cap_of(k, nt * u)) + 4 * (size_t)nt; }
+  // ROOM tiles' pieces behind twice what is kept; behind the pieces kept all their columns, which is also what 8 slices keep
+  static constexpr int ROOM = 4;
+  static __host__ __device__ int most(int k) { return k + slack_of(k); }
+  static __host__ __device__ int cap_of(int k, int tile) { return max(ROOM * tile + 2 * most(k), 9 * most(k)); }
+  static size_t shared_bytes(int k, int nt, int u) { return sizeof(Head) + 8 * ((size_t)most(k) + cap_of(k, nt * u)) + 4 * (size_t)nt; }
   __device__ __forceinline__ TopK(unsigned char* at, int k_, int tile)
-      : h(*reinterpret_cast<Head*>(at)), kept(reinterpret_cast<unsigned long long*>(at + sizeof(Head))), piece(kept + k_ + slack_of(k_)),
+      : h(*reinterpret_cast<Head*>(at)), kept(reinterpret_cast<unsigned long long*>(at + sizeof(Head))), piece(kept + most(k_)),
         top(reinterpret_cast<uint32_t*>(piece + cap_of(k_, tile))), k(k_), cap(cap_of(k_, tile)) {}
+  __device__ __forceinline__ unsigned long long* column_list() const { return piece + most(k); }
 };
 
-// The largest bound that at least k (at most k + slack, unless equal keys forbid) of n keys reach; one warp, keys `step` words apart.
-__device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int step, int k, int slack, int* reach) {
+template <int NT> __device__ __forceinline__ void sync() { if (NT == 32) __syncwarp(); else __syncthreads(); }
+template <int NT> __device__ __forceinline__ int sync_or(int v) { return NT == 32 ? __any_sync(0xffffffffu, v) : __syncthreads_or(v); }
+
+// Appends the keys that the lanes bring (those of `key` whose bit is set), in no fixed order; one atomic per warp: 32 lanes on one
+// counter would take their turns.  The count behind this warp's keys (0: it brought none).
+template <int N>
+__device__ __forceinline__ int append(unsigned long long* to, int* count, uint32_t mine, const unsigned long long (&key)[N]) {
+  const int lane = threadIdx.x & 31, n = __popc(mine);
+  int upto = n;
+  if (N == 1) {
+    upto = __popc(__ballot_sync(0xffffffffu, n) & (0xffffffffu >> (31 - lane)));
+  } else {
+    if (!__any_sync(0xffffffffu, n)) return 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+  }
+  int at = 0;
+  if (lane == 31 && upto > 0) at = atomicAdd(count, upto);
+  at = __shfl_sync(0xffffffffu, at, 31);
+  const int all = __shfl_sync(0xffffffffu, upto, 31);
+  if (all == 0) return 0;
+  int put = at + upto - n;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (mine >> i & 1) to[put++] = key[i];
+  return at + all;
+}
+
+// The largest bound that at least k (at most k + slack, unless equal keys forbid) of n keys reach; one warp, keys STEP words apart.
+// SHIFT: the low bits of a key that say nothing (a 16-bit logit's are all 0 or all 1), not searched.
+template <int SHIFT, int STEP>
+__device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int k, int slack, int* reach) {
+  constexpr int HELD = 8;                                // keys a lane has in registers; more are read again
   const int lane = threadIdx.x & 31;
-  uint32_t lo = 0xffffffffu, hi = 0;
-  for (int i = lane; i < n; i += 32) { lo = min(lo, keys[i * step]); hi = max(hi, keys[i * step]); }
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi) + 1;           // (no key is ~0)
+  uint32_t held[HELD], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int u = 0; u < HELD; ++u) {
+    const int i = lane + 32 * u;
+    held[u] = i < n ? keys[i * STEP] : 0;                // (0 is below every bound)
+    if (i < n) { lo = min(lo, held[u]); hi = max(hi, held[u]); }
+  }
+  for (int i = lane + 32 * HELD; i < n; i += 32) { lo = min(lo, keys[i * STEP]); hi = max(hi, keys[i * STEP]); }
+  lo = __reduce_min_sync(0xffffffffu, lo) >> SHIFT;
+  hi = (__reduce_max_sync(0xffffffffu, hi) >> SHIFT) + 1;            // (no key is ~0)
   int at_lo = n;
   while (hi - lo > 1 && at_lo > k + slack) {
-    const uint32_t mid = lo + (hi - lo) / 2;
+    const uint32_t mid = lo + (hi - lo) / 2, bound = mid << SHIFT;
     int c = 0;
-#pragma unroll 4
-    for (int i = lane; i < n; i += 32) c += keys[i * step] >= mid;
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) c += held[u] >= bound;
+    for (int i = lane + 32 * HELD; i < n; i += 32) c += keys[i * STEP] >= bound;
     c = __reduce_add_sync(0xffffffffu, c);
     if (c >= k) { lo = mid; at_lo = c; } else hi = mid;
   }
   *reach = at_lo;
-  return lo;
+  return lo << SHIFT;
 }
 
-// A bound that at least k and at most k + slack of n distinct keys reach (0: all), by one warp.
-__device__ unsigned long long warp_bound64(const unsigned long long* keys, int n, int k, int slack) {
-  if (n <= k + slack) return 0;
+// A bound that at least k and at most k + slack of n distinct keys reach, n > k + slack; one warp.
+template <int SHIFT>
+__device__ __noinline__ unsigned long long warp_bound64(const unsigned long long* keys, int n, int k, int slack) {
   const int lane = threadIdx.x & 31;
   int reach;
-  const uint32_t value = warp_bound(reinterpret_cast<const uint32_t*>(keys) + 1, n, 2, k, slack, &reach);
+  const uint32_t value = warp_bound<SHIFT, 2>(reinterpret_cast<const uint32_t*>(keys) + 1, n, k, slack, &reach);
   if (reach <= k + slack) return (unsigned long long)value << 32;
   int above = 0;                                         // many equal values at the end: the lowest of their columns
-  for (int i = lane; i < n; i += 32) above += uint32_t(keys[i] >> 32) > value;
+  uint32_t same = 0;                                     // (their key, with the bits that were not searched)
+  for (int i = lane; i < n; i += 32)
+    if (uint32_t(keys[i] >> 32) >> SHIFT == value >> SHIFT) same = uint32_t(keys[i] >> 32);
+  same = __reduce_max_sync(0xffffffffu, same);
+  for (int i = lane; i < n; i += 32) above += uint32_t(keys[i] >> 32) > same;
   const int want = k - __reduce_add_sync(0xffffffffu, above);
   unsigned long long lo = 0, hi = 1ull << 32;
   int at_lo = reach - (k - want);
   while (hi - lo > 1 && at_lo > want + slack) {
     const unsigned long long mid = lo + (hi - lo) / 2;
     int c = 0;
-    for (int i = lane; i < n; i += 32) c += uint32_t(keys[i] >> 32) == value && uint32_t(keys[i]) >= mid;
+    for (int i = lane; i < n; i += 32) c += uint32_t(keys[i] >> 32) == same && uint32_t(keys[i]) >= mid;
     c = __reduce_add_sync(0xffffffffu, c);
     if (c >= want) { lo = mid; at_lo = c; } else hi = mid;
   }
-  return (unsigned long long)value << 32 | lo;
+  return (unsigned long long)same << 32 | lo;
 }
 
-// kept = those of the first `count` keys that reach a bound which k to k + slack of them reach (all, if there are no more); keep: how many.
-template <int NT>
-__device__ __forceinline__ void thin(TopK& S) {
-  __syncthreads();
-  const int n = S.h.count;
+// kept = those of n > k + slack keys that reach a bound which k to k + slack of them reach; keep: how many.  Everyone is past writing them.
+template <int NT, int SHIFT>
+__device__ __forceinline__ void thin(TopK& S, const unsigned long long* keys, int n) {
   if (threadIdx.x < 32) {
-    const unsigned long long b = warp_bound64(S.piece, n, S.k, slack_of(S.k));
+    const unsigned long long b = warp_bound64<SHIFT>(keys, n, S.k, slack_of(S.k));
     if (threadIdx.x == 0) { S.h.bound = b > S.h.bound ? b : S.h.bound; S.h.keep = 0; }
   }
-  __syncthreads();
+  sync<NT>();
   const unsigned long long b = S.h.bound;
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const unsigned long long key = S.piece[i];
-    if (key >= b) S.kept[atomicAdd(&S.h.keep, 1)] = key;
+  for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += NT) {
+    const unsigned long long key[1] = {i < n ? keys[i] : 0};
+    append<1>(S.kept, &S.h.keep, i < n && key[0] >= b, key);
   }
-  __syncthreads();
+  sync<NT>();
 }
 
 // Notes a tile's pieces (top[u]: the largest of piece first + u * NT, below `end`; all: of this thread's) that reach the bound.  Whether
-// this thread found no room for another tile behind its own.
-template <int NT, int U>
+// there is no room for another tile behind them.
+template <int NT, int U, int SHIFT>
 __device__ __forceinline__ bool note(TopK& S, const float (&top)[U], float all, int first, int end, bool start) {
   const int tid = threadIdx.x;
   if (start) {
     const int n = min(end - (first - tid), NT);          // threads with a piece
     S.top[tid] = value_key(all);
     if (tid == 0) S.h.count = 0;
-    __syncthreads();
+    sync<NT>();
     if (tid < 32) {
       int reach;
-      const uint32_t b = n > S.k ? warp_bound(S.top, n, 1, S.k, S.k / 8, &reach) : 0;
+      const uint32_t b = n > S.k ? warp_bound<SHIFT, 1>(S.top, n, S.k, S.k / 4 + 4, &reach) : 0;
       if (tid == 0) S.h.bound = (unsigned long long)b << 32;
     }
-    __syncthreads();
+    sync<NT>();
   }
   const unsigned long long bound = S.h.bound;
   const float least = key_value(bound);                  // (NaN: no bound, or NaN is)
-  int last = -1;
+  unsigned long long key[U];
+  uint32_t mine = 0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (first + u * NT >= end || top[u] < least) continue;
-    const unsigned long long key = order_key(top[u], first + u * NT);
-    if (key >= bound) S.piece[last = atomicAdd(&S.h.count, 1)] = key;
+    key[u] = order_key(top[u], first + u * NT);
+    if (first + u * NT < end && !(top[u] < least) && key[u] >= bound) mine |= 1u << u;
   }
-  return last >= S.cap - NT * U;
+  return append<U>(S.piece, &S.h.count, mine, key) > S.cap - TopK::ROOM * NT * U;
 }
-// Behind a tile that another one follows: room for all of its pieces.
-template <int NT>
+// Room for the pieces of ROOM tiles.
+template <int NT, int SHIFT>
 __device__ __forceinline__ void make_room(TopK& S, bool full) {
-  if (!__syncthreads_or(full)) return;                   // (the count itself may grow while others still look)
-  thin<NT>(S);
+  if (!sync_or<NT>(full)) return;                        // (the count itself may grow while others still look)
+  thin<NT, SHIFT>(S, S.piece, S.h.count);
   const int n = S.h.keep;
   for (int i = threadIdx.x; i < n; i += NT) S.piece[i] = S.kept[i];
   if (threadIdx.x == 0) S.h.count = n;
-  __syncthreads();
+  sync<NT>();
 }
-// In the end: kept = columns among which the row's (the slice's) k largest logits are, `keep` of them, no more than k + slack.
+// The keys at `from` (0: kept, 1: column_list), if they are many thinned out into `kept`.
+template <int NT, int SHIFT>
+__device__ __forceinline__ void shorten(TopK& S) {
+  sync<NT>();
+  const int n = S.h.count;
+  if (n > TopK::most(S.k)) {
+    thin<NT, SHIFT>(S, S.column_list(), n);
+    if (threadIdx.x == 0) S.h.from = 0;
+  } else if (threadIdx.x == 0) {
+    S.h.keep = n;
+    S.h.from = 1;
+  }
+  sync<NT>();
+}
+// In the end: `keep` columns at `from` among which the row's (the slice's) k largest logits are, no more than k + slack.
 template <typename T, int NT>
 __device__ __forceinline__ void columns(TopK& S, const Row<T>& row) {
   constexpr int N = Vec<T>::N;
-  thin<NT>(S);
-  const int pieces = S.h.keep;
-  const unsigned long long bound = S.h.bound & 0xffffffff00000000ull;     // (of k pieces' largest: k columns reach its value)
-  __syncthreads();
-  if (threadIdx.x == 0) { S.h.count = 0; S.h.bound = bound; }
-  __syncthreads();
-  for (int i = threadIdx.x; i < pieces * N; i += NT) {
-    const int c = row.column((int)~(uint32_t)S.kept[i / N]) + i % N;
-    if (c < 0 || c >= row.V) continue;
-    const unsigned long long key = order_key(row.at(c), c);
-    if (key >= bound) S.piece[atomicAdd(&S.h.count, 1)] = key;
+  sync<NT>();
+  int n = S.h.count;
+  const unsigned long long* from = S.piece;
+  if (n > TopK::most(S.k)) {
+    thin<NT, Vec<T>::SHIFT>(S, S.piece, n);
+    n = S.h.keep;
+    from = S.kept;
   }
-  thin<NT>(S);
+  const unsigned long long bound = S.h.bound & 0xffffffff00000000ull;     // (of k pieces' largest: k columns reach its value)
+  sync<NT>();
+  if (threadIdx.x == 0) { S.h.count = 0; S.h.bound = bound; }
+  sync<NT>();
+#pragma unroll 2
+  for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += NT) {
+    unsigned long long key[N] = {};
+    uint32_t mine = 0;
+    if (i < n) {
+      const int v = (int)~(uint32_t)from[i], c = row.column(v);
+      float x[N];
+      Vec<T>::unpack(row.load(v), x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        key[j] = order_key(x[j], c + j);
+        if (key[j] >= bound && c + j >= 0 && c + j < row.V) mine |= 1u << j;
+      }
+    }
+    append<N>(S.column_list(), &S.h.count, mine, key);
+  }
+  shorten<NT, Vec<T>::SHIFT>(S);
 }
 
 // ---------------------------------------------------------------- one pass over a row's pieces [begin, end)
@@ -328,6 +408,7 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
   constexpr int N = Vec<T>::N, TILE = NT * U;
   const int tid = threadIdx.x;
   Sums a = no_sums();
+  bool more = false;
   for (int tile = begin; tile < end; tile += TILE) {
     const int first = tile + tid;
     uint4 raw[U];
@@ -383,8 +464,9 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
     a.s += s[0];
     if (ENTROPY) a.e += e[0] + e[1];
     if (TOP) {
-      const bool full = note<NT, U>(*top_k, top, all, first, end, tile == begin);
-      if (tile + TILE < end) make_room<NT>(*top_k, full);
+      const bool full = note<NT, U, Vec<T>::SHIFT>(*top_k, top, all, first, end, tile == begin);
+      more |= full;                                              // (looked at by all threads every ROOM tiles)
+      if (tile + TILE < end && ((tile - begin) / TILE + 1) % TopK::ROOM == 0) { make_room<NT, Vec<T>::SHIFT>(*top_k, more); more = false; }
     }
   }
   return a;
@@ -411,7 +493,7 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
 // ---------------------------------------------------------------- forward
 // A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.
 template <typename T, int NT, int U, bool TOP>
-__global__ void __launch_bounds__(NT, 1280 / NT > 20 ? 20 : 1280 / NT)
+__global__ void __launch_bounds__(NT, NT == 32 ? TS_MB32 : TS_MB128 * 128 / NT)
 token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, double inv_t, int k, float* __restrict__ logprob,
                       float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids, float2* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
@@ -438,7 +520,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   a = block_sums<NT>(a, red);
   if (TOP) {
     if (begin < end) columns<T, NT>(top, row);
-    else if (tid == 0) { top.h.keep = 0; top.h.bound = 0; }
+    else if (tid == 0) { top.h.keep = 0; top.h.from = 0; top.h.bound = 0; }
   }
   if (C > 1) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -463,17 +545,19 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
       a.s = a.e = 0.f;
       for (int r = 0; r < C; ++r) { const Sums* o = cluster.map_shared_rank(&mine, r); a.s += o->s; a.e += o->e; }
     }
-    if (TOP && rank == 0) {
-      int n = 0;
-      for (int r = 0; r < C; ++r) {
-        const unsigned long long* kept = cluster.map_shared_rank(top.kept, r);
-        const int m = cluster.map_shared_rank(&top.h, r)->keep;
-        for (int i = tid; i < m; i += NT) top.piece[n + i] = kept[i];
+    if (TOP && rank == 0) {                                      // the others' lists behind this CTA's
+      int n = top.h.keep;
+      if (!top.h.from) for (int i = tid; i < n; i += NT) top.column_list()[i] = top.kept[i];
+      for (int r = 1; r < C; ++r) {
+        const TopK::Head* h = cluster.map_shared_rank(&top.h, r);
+        const unsigned long long* list = cluster.map_shared_rank(h->from ? top.column_list() : top.kept, r);
+        const int m = h->keep;
+        for (int i = tid; i < m; i += NT) top.column_list()[n + i] = list[i];
         n += m;
       }
-      if (tid == 0) top.h.count = n;
       cluster.sync();                                            // (the others leave)
-      thin<NT>(top);
+      if (tid == 0) top.h.count = n;
+      shorten<NT, Vec<T>::SHIFT>(top);
     } else {
       cluster.sync();
     }
@@ -482,6 +566,9 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
     a = sums_far<T, NT, false>(row, begin, end, a.top, c, nullptr, 0, red);
   }
   const bool none = a.s == 0.f;                                  // nothing but -inf
+  const int n = TOP ? top.h.keep : 0;
+  const unsigned long long* list = TOP && top.h.from ? top.column_list() : top.kept;
+  if (tid >= max(n, 1)) return;
   const RowSum sum(a, c);
   if (tid == 0) {
     logprob[row_at] = none ? -INFINITY : (float)sum.logprob(target, inv_t);
@@ -489,13 +576,16 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
     entropy[row_at] = none ? 0.f : LN2 * (log2f(a.s) - a.e / a.s);
     stats[row_at] = make_float2(a.top, none ? -INFINITY : log2f(a.s));
   }
-  if (!TOP) return;
-  const int n = top.h.keep;
   for (int i = tid; i < n; i += NT) {                            // the list's order: how many keys come before
-    const unsigned long long key = top.kept[i];
+    const unsigned long long key = list[i];
     int before = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) before += top.kept[j] > key;
+    for (int j = 0; j + 1 < n; j += 2) {                         // (the lists start on 16 bytes)
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + j);
+      before += two.x > key;
+      before += two.y > key;
+    }
+    if (n & 1) before += list[n - 1] > key;
     if (before >= k) continue;
     top_ids[row_at * k + before] = (int)~(uint32_t)key;
     top_lp[row_at * k + before] = none ? -INFINITY : (float)sum.logprob(key_value(key), inv_t);
@@ -659,11 +749,12 @@ struct Slice {
 #pragma unroll
     for (int i = 0; i < Vec<T>::N; ++i) if (c + i >= 0 && c + i < row.V) dx[c + i] = Vec<T>::from_f(y[i]);
   }
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    uint4 raw[U];
+  __device__ __forceinline__ void load(uint4 (&raw)[U]) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) if (first + u * NT < end) raw[u] = row.load(first + u * NT);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(const uint4 (&raw)[U], F f) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (first + u * NT >= end) break;
@@ -693,6 +784,8 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const int6
   const float2 st = stats[row_at];
   const Slice<T, NT, U> slice(logits + row_at * ld, dlogits + row_at * V, V, part);
   if (tok < 0 || tok >= V || st.y == -INFINITY) return slice.zero();
+  uint4 raw[U];                                                  // (requested ahead of what depends on other loads)
+  slice.load(raw);
   const float g = g_lp ? g_lp[row_at] : 0.f, gh = g_h ? g_h[row_at] : 0.f;
   float all = g;
   if (!g_top) k = 0;
@@ -718,7 +811,7 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const int6
     const float l = ex(x) - st.y;
     return exp2_fast(l) * fmaf(b, weighted(l), a);
   };
-  slice.each(base);
+  slice.each(raw, base);
   __syncthreads();
   for (int i = tid; i < k; i += NT) {
     const long long j = top_ids[row_at * k + i];
@@ -743,6 +836,8 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
   const float4 st = stats[row_at * 2], list = stats[row_at * 2 + 1];
   const Slice<T, NT, U> slice(logits + row_at * ld, dlogits + row_at * V, V, part);
   if (st.w == 0.f) return slice.zero();
+  uint4 raw[U];
+  slice.load(raw);
   for (int i = tid; i < k; i += NT) {
     const long long j = ids[row_at * k + i];
     id[i] = slice.holds(j, part) ? (int)j : -1;
@@ -750,7 +845,7 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
   }
   const Exponent ex(st.x, c);
   const float scale = dloss[row_at] * temp, outside = scale * st.z, inside = scale * st.w;
-  slice.each([&](float x) { return exp2_fast(ex(x) - st.y) * outside; });
+  slice.each(raw, [&](float x) { return exp2_fast(ex(x) - st.y) * outside; });
   __syncthreads();
   for (int i = tid; i < k; i += NT) {
     if (id[i] < 0) continue;
@@ -795,17 +890,30 @@ int pieces_of(const void* x, int type, long long ld, int V) {
 }
 
 // A row of at most one tile of 32 or 128 threads is one CTA of them; longer ones are walked by 256.
-#define BY_SIZE(T, pieces, CALL)          \
-  do {                                    \
-    if (pieces <= 128) CALL(T, 32, 4);    \
-    else if (pieces <= 512) CALL(T, 128, 4); \
-    else CALL(T, 256, 4);                 \
+#ifndef TS_FEW
+#define TS_FEW 2960
+#define TS_NB 128
+#define TS_WIDE 296
+#endif
+// Forward: a row of up to four tiles of a warp is that warp's where there are rows enough, others are walked by 128 threads.
+#define FORWARD(T, rows, pieces, CALL)                        \
+  do {                                                        \
+    if (pieces <= 128 || (pieces <= 512 && rows >= TS_FEW)) CALL(T, 32, 4); \
+    else if (rows >= TS_WIDE || pieces <= 512) CALL(T, 128, 4);                                     \
+    else CALL(T, 256, 4);                                     \
   } while (0)
-#define BY_TYPE_AND_SIZE(type, pieces, CALL)                      \
-  do {                                                            \
-    if (type == RTE_TYPE_BF16) BY_SIZE(__nv_bfloat16, pieces, CALL); \
-    else if (type == RTE_TYPE_F16) BY_SIZE(__half, pieces, CALL); \
-    else BY_SIZE(float, pieces, CALL);                            \
+// Backward: as many threads as four pieces each cover the row with, up to 256.
+#define BACKWARD(T, rows, pieces, CALL)     \
+  do {                                      \
+    if (pieces <= 128) CALL(T, 32, 4);      \
+    else if (pieces <= 512) CALL(T, 128, 4); \
+    else CALL(T, TS_NB, 4);                   \
+  } while (0)
+#define BY_TYPE(type, WHICH, rows, pieces, CALL)                              \
+  do {                                                                        \
+    if (type == RTE_TYPE_BF16) WHICH(__nv_bfloat16, rows, pieces, CALL);      \
+    else if (type == RTE_TYPE_F16) WHICH(__half, rows, pieces, CALL);         \
+    else WHICH(float, rows, pieces, CALL);                                    \
   } while (0)
 
 bool temperature_ok(float t) { return t >= 1e-30f && t <= 1e30f; }
@@ -834,7 +942,7 @@ extern "C" int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t 
                    tokens, (long long)ignore_index, log2_scale(temperature), 1. / temperature, (int)top_k, logprob, entropy, top_logprobs,    \
                    top_ids, reinterpret_cast<float2*>(row_stats), (int)V, C, status);                                                                        \
   } while (0)
-  BY_TYPE_AND_SIZE(type, pieces, CALL);
+  BY_TYPE(type, FORWARD, rows, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -855,7 +963,7 @@ extern "C" int rte_token_logprobs_bwd(const void* logits, int32_t type, int64_t 
                 1.f / temperature, top_k, top_ids, reinterpret_cast<const float2*>(row_stats), entropy, g_logprob, g_entropy, g_top, static_cast<T*>(dlogits), V, \
                 parts);                                                                                                                                       \
   } while (0)
-  BY_TYPE_AND_SIZE(type, pieces, CALL);
+  BY_TYPE(type, BACKWARD, rows, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -874,7 +982,7 @@ extern "C" int rte_distill_topk_fwd(const void* logits, int32_t type, int64_t ld
                    static_cast<const T*>(logits), (long long)ldl, teacher, ids, (int)k, log2_scale(temperature), (double)temperature, loss,                    \
                    reinterpret_cast<float4*>(row_stats), (int)V, C, status);                                                                                   \
   } while (0)
-  BY_TYPE_AND_SIZE(type, pieces, CALL);
+  BY_TYPE(type, FORWARD, rows, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -893,7 +1001,7 @@ extern "C" int rte_distill_topk_bwd(const void* logits, int32_t type, int64_t ld
     rte::launch(distill_topk_bwd_kernel<T, NT, U>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, teacher, ids, k, log2_scale(temperature), \
                 temperature, reinterpret_cast<const float4*>(row_stats), dloss, static_cast<T*>(dlogits), V, parts);                                          \
   } while (0)
-  BY_TYPE_AND_SIZE(type, pieces, CALL);
+  BY_TYPE(type, BACKWARD, rows, pieces, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
