@@ -22,6 +22,7 @@ namespace {
 #ifndef TS_MB32
 #define TS_MB32 24
 #define TS_MB128 10
+#define TS_R128 2
 #endif
 constexpr int TS_MAX_LIST = RTE_TOKEN_LIST_MAX;
 constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
@@ -169,7 +170,6 @@ struct RowSum {
     shift = careful(a) || !(fabsf(a.R) < FAR) ? 0. : (double)a.top * c - a.R;
     ln_s = log((double)a.s) - shift * LN2_D;
   }
-  __device__ __forceinline__ double logprob(float x, double inv_t) const { return (x - top) * inv_t - ln_s; }
 };
 
 // The exponent of a logit relative to the row's largest, as forward formed it; p = 2^(t - l2) with l2 as forward kept it.
@@ -203,60 +203,59 @@ struct TopK {                                            // in shared memory, si
   unsigned long long *kept, *piece;                      // [k + slack], [cap]: value | ~piece; from piece + k + slack on, in the end: value | ~column
   uint32_t* top;                                         // [threads]
   int k, cap;
-  // ROOM tiles' pieces behind twice what is kept; behind the pieces kept all their columns, which is also what 8 slices keep
-  static constexpr int ROOM = 4;
+  // a round's pieces behind twice what is kept; behind the pieces kept all their columns, which is also what 8 slices keep
   static __host__ __device__ int most(int k) { return k + slack_of(k); }
-  static __host__ __device__ int cap_of(int k, int tile) { return max(ROOM * tile + 2 * most(k), 9 * most(k)); }
-  static size_t shared_bytes(int k, int nt, int u) { return sizeof(Head) + 8 * ((size_t)most(k) + cap_of(k, nt * u)) + 4 * (size_t)nt; }
-  __device__ __forceinline__ TopK(unsigned char* at, int k_, int tile)
+  static __host__ __device__ int cap_of(int k, int round) { return max(round + 2 * most(k), 9 * most(k)); }
+  static size_t shared_bytes(int k, int nt, int round) { return sizeof(Head) + 8 * ((size_t)most(k) + cap_of(k, round)) + 4 * ((size_t)nt + round); }
+  float* tops;                                           // [round]: the largest of every piece of a round, each its thread's own
+  __device__ __forceinline__ TopK(unsigned char* at, int k_, int nt, int round)
       : h(*reinterpret_cast<Head*>(at)), kept(reinterpret_cast<unsigned long long*>(at + sizeof(Head))), piece(kept + most(k_)),
-        top(reinterpret_cast<uint32_t*>(piece + cap_of(k_, tile))), k(k_), cap(cap_of(k_, tile)) {}
+        top(reinterpret_cast<uint32_t*>(piece + cap_of(k_, round))), k(k_), cap(cap_of(k_, round)), tops(reinterpret_cast<float*>(top + nt)) {}
   __device__ __forceinline__ unsigned long long* column_list() const { return piece + most(k); }
 };
+// Tiles whose pieces' maxima are kept before they are looked through: 512 pieces or 2048.
+__host__ __device__ constexpr int round_tiles(int nt) { return nt == 256 ? 2 : nt == 128 ? TS_R128 : 4; }
 
 template <int NT> __device__ __forceinline__ void sync() { if (NT == 32) __syncwarp(); else __syncthreads(); }
 template <int NT> __device__ __forceinline__ int sync_or(int v) { return NT == 32 ? __any_sync(0xffffffffu, v) : __syncthreads_or(v); }
 
-// Appends the keys that the lanes bring (those of `key` whose bit is set), in no fixed order; one atomic per warp: 32 lanes on one
-// counter would take their turns.  The count behind this warp's keys (0: it brought none).
-template <int N>
-__device__ __forceinline__ int append(unsigned long long* to, int* count, uint32_t mine, const unsigned long long (&key)[N]) {
-  const int lane = threadIdx.x & 31, n = __popc(mine);
+// Room in a list for the n keys that each lane brings: where this lane's begin, and the count behind the warp's (0: it brings
+// none).  One atomic per warp: 32 lanes on one counter would take their turns.
+__device__ __forceinline__ int2 reserve(int* count, int n) {
+  const int lane = threadIdx.x & 31;
+  if (!__any_sync(0xffffffffu, n)) return make_int2(0, 0);
   int upto = n;
-  if (N == 1) {
-    upto = __popc(__ballot_sync(0xffffffffu, n) & (0xffffffffu >> (31 - lane)));
-  } else {
-    if (!__any_sync(0xffffffffu, n)) return 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
-  }
+  for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
   int at = 0;
-  if (lane == 31 && upto > 0) at = atomicAdd(count, upto);
+  if (lane == 31) at = atomicAdd(count, upto);
   at = __shfl_sync(0xffffffffu, at, 31);
-  const int all = __shfl_sync(0xffffffffu, upto, 31);
-  if (all == 0) return 0;
-  int put = at + upto - n;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (mine >> i & 1) to[put++] = key[i];
-  return at + all;
+  return make_int2(at + upto - n, at + __shfl_sync(0xffffffffu, upto, 31));
+}
+__device__ __forceinline__ void append(unsigned long long* to, int* count, bool mine, unsigned long long key) {
+  const uint32_t who = __ballot_sync(0xffffffffu, mine);
+  if (who == 0) return;
+  int at = 0;
+  if ((threadIdx.x & 31) == 0) at = atomicAdd(count, __popc(who));
+  at = __shfl_sync(0xffffffffu, at, 0);
+  if (mine) to[at + __popc(who & ((1u << (threadIdx.x & 31)) - 1))] = key;
 }
 
 // The largest bound that at least k (at most k + slack, unless equal keys forbid) of n keys reach; one warp, keys STEP words apart.
 // SHIFT: the low bits of a key that say nothing (a 16-bit logit's are all 0 or all 1), not searched.
-template <int SHIFT, int STEP>
+template <int SHIFT, int STEP, int HELD>                 // HELD: keys a lane has in registers; more are read again
 __device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int k, int slack, int* reach) {
-  constexpr int HELD = 8;                                // keys a lane has in registers; more are read again
   const int lane = threadIdx.x & 31;
   uint32_t held[HELD], lo = 0xffffffffu, hi = 0;
 #pragma unroll
   for (int u = 0; u < HELD; ++u) {
     const int i = lane + 32 * u;
     held[u] = i < n ? keys[i * STEP] : 0;                // (0 is below every bound)
-    if (i < n) { lo = min(lo, held[u]); hi = max(hi, held[u]); }
+    lo = min(lo, held[u] - 1);                           // (and its predecessor above all)
+    hi = max(hi, held[u]);
   }
-  for (int i = lane + 32 * HELD; i < n; i += 32) { lo = min(lo, keys[i * STEP]); hi = max(hi, keys[i * STEP]); }
-  lo = __reduce_min_sync(0xffffffffu, lo) >> SHIFT;
+  for (int i = lane + 32 * HELD; i < n; i += 32) { lo = min(lo, keys[i * STEP] - 1); hi = max(hi, keys[i * STEP]); }
+  lo = (__reduce_min_sync(0xffffffffu, lo) + 1) >> SHIFT;
   hi = (__reduce_max_sync(0xffffffffu, hi) >> SHIFT) + 1;            // (no key is ~0)
   int at_lo = n;
   while (hi - lo > 1 && at_lo > k + slack) {
@@ -277,7 +276,8 @@ template <int SHIFT>
 __device__ __noinline__ unsigned long long warp_bound64(const unsigned long long* keys, int n, int k, int slack) {
   const int lane = threadIdx.x & 31;
   int reach;
-  const uint32_t value = warp_bound<SHIFT, 2>(reinterpret_cast<const uint32_t*>(keys) + 1, n, k, slack, &reach);
+  const uint32_t* values = reinterpret_cast<const uint32_t*>(keys) + 1;
+  const uint32_t value = n <= 128 ? warp_bound<SHIFT, 2, 4>(values, n, k, slack, &reach) : warp_bound<SHIFT, 2, 16>(values, n, k, slack, &reach);
   if (reach <= k + slack) return (unsigned long long)value << 32;
   int above = 0;                                         // many equal values at the end: the lowest of their columns
   uint32_t same = 0;                                     // (their key, with the bits that were not searched)
@@ -300,24 +300,25 @@ __device__ __noinline__ unsigned long long warp_bound64(const unsigned long long
 
 // kept = those of n > k + slack keys that reach a bound which k to k + slack of them reach; keep: how many.  Everyone is past writing them.
 template <int NT, int SHIFT>
-__device__ __forceinline__ void thin(TopK& S, const unsigned long long* keys, int n) {
+__device__ __forceinline__ void thin(TopK& S, const unsigned long long* keys, int n, int slack) {
   if (threadIdx.x < 32) {
-    const unsigned long long b = warp_bound64<SHIFT>(keys, n, S.k, slack_of(S.k));
+    const unsigned long long b = warp_bound64<SHIFT>(keys, n, S.k, slack);
     if (threadIdx.x == 0) { S.h.bound = b > S.h.bound ? b : S.h.bound; S.h.keep = 0; }
   }
   sync<NT>();
   const unsigned long long b = S.h.bound;
   for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += NT) {
-    const unsigned long long key[1] = {i < n ? keys[i] : 0};
-    append<1>(S.kept, &S.h.keep, i < n && key[0] >= b, key);
+    const unsigned long long key = i < n ? keys[i] : 0;
+    append(S.kept, &S.h.keep, i < n && key >= b, key);
   }
   sync<NT>();
 }
 
-// Notes a tile's pieces (top[u]: the largest of piece first + u * NT, below `end`; all: of this thread's) that reach the bound.  Whether
-// there is no room for another tile behind them.
-template <int NT, int U, int SHIFT>
-__device__ __forceinline__ bool note(TopK& S, const float (&top)[U], float all, int first, int end, bool start) {
+// Looks through a round: notes those of this thread's pieces (tops[j * NT + tid]: the largest of piece first + j * NT, below `end`) that
+// reach the bound.  all: the largest of them.  Leaves room for another round where one follows.
+template <int NT, int COUNT, int SHIFT>
+__device__ __forceinline__ void note(TopK& S, float all, int first, int end, bool start) {
+  constexpr int round = NT * COUNT;
   const int tid = threadIdx.x;
   if (start) {
     const int n = min(end - (first - tid), NT);          // threads with a piece
@@ -326,30 +327,32 @@ __device__ __forceinline__ bool note(TopK& S, const float (&top)[U], float all, 
     sync<NT>();
     if (tid < 32) {
       int reach;
-      const uint32_t b = n > S.k ? warp_bound<SHIFT, 1>(S.top, n, S.k, S.k / 4 + 4, &reach) : 0;
+      const uint32_t b = n > S.k ? warp_bound<SHIFT, 1, NT / 32>(S.top, n, S.k, S.k / 8, &reach) : 0;
       if (tid == 0) S.h.bound = (unsigned long long)b << 32;
     }
     sync<NT>();
   }
   const unsigned long long bound = S.h.bound;
   const float least = key_value(bound);                  // (NaN: no bound, or NaN is)
-  unsigned long long key[U];
   uint32_t mine = 0;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    key[u] = order_key(top[u], first + u * NT);
-    if (first + u * NT < end && !(top[u] < least) && key[u] >= bound) mine |= 1u << u;
+  for (int j = 0; j < COUNT; ++j)
+    if (!(S.tops[j * NT + tid] < least)) mine |= 1u << j;
+  const int have = first < end ? min((end - first + NT - 1) / NT, COUNT) : 0;
+  mine &= (1u << have) - 1;
+  int2 at = reserve(&S.h.count, __popc(mine));
+  const bool full = at.y > S.cap - round;
+  while (mine) {
+    const int j = __ffs(mine) - 1;
+    mine &= mine - 1;
+    S.piece[at.x++] = order_key(S.tops[j * NT + tid], first + j * NT);
   }
-  return append<U>(S.piece, &S.h.count, mine, key) > S.cap - TopK::ROOM * NT * U;
-}
-// Room for the pieces of ROOM tiles.
-template <int NT, int SHIFT>
-__device__ __forceinline__ void make_room(TopK& S, bool full) {
-  if (!sync_or<NT>(full)) return;                        // (the count itself may grow while others still look)
-  thin<NT, SHIFT>(S, S.piece, S.h.count);
-  const int n = S.h.keep;
-  for (int i = threadIdx.x; i < n; i += NT) S.piece[i] = S.kept[i];
-  if (threadIdx.x == 0) S.h.count = n;
+  if (first - tid + round >= end || !sync_or<NT>(full)) return;      // (the count itself may grow while others still look)
+  const int n = S.h.count;
+  thin<NT, SHIFT>(S, S.piece, n, slack_of(S.k));
+  const int keep = S.h.keep;
+  for (int i = tid; i < keep; i += NT) S.piece[i] = S.kept[i];
+  if (tid == 0) S.h.count = keep;
   sync<NT>();
 }
 // The keys at `from` (0: kept, 1: column_list), if they are many thinned out into `kept`.
@@ -357,8 +360,8 @@ template <int NT, int SHIFT>
 __device__ __forceinline__ void shorten(TopK& S) {
   sync<NT>();
   const int n = S.h.count;
-  if (n > TopK::most(S.k)) {
-    thin<NT, SHIFT>(S, S.column_list(), n);
+  if (n > S.k + S.k / 8 + 8) {                             // (they are ordered by counting: n^2 comparisons)
+    thin<NT, SHIFT>(S, S.column_list(), n, S.k / 8 + 8);
     if (threadIdx.x == 0) S.h.from = 0;
   } else if (threadIdx.x == 0) {
     S.h.keep = n;
@@ -374,7 +377,7 @@ __device__ __forceinline__ void columns(TopK& S, const Row<T>& row) {
   int n = S.h.count;
   const unsigned long long* from = S.piece;
   if (n > TopK::most(S.k)) {
-    thin<NT, Vec<T>::SHIFT>(S, S.piece, n);
+    thin<NT, Vec<T>::SHIFT>(S, S.piece, n, slack_of(S.k));
     n = S.h.keep;
     from = S.kept;
   }
@@ -382,21 +385,25 @@ __device__ __forceinline__ void columns(TopK& S, const Row<T>& row) {
   sync<NT>();
   if (threadIdx.x == 0) { S.h.count = 0; S.h.bound = bound; }
   sync<NT>();
+  const float least = key_value(bound);
 #pragma unroll 2
   for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += NT) {
-    unsigned long long key[N] = {};
+    float x[N];
     uint32_t mine = 0;
+    int c = 0;
     if (i < n) {
-      const int v = (int)~(uint32_t)from[i], c = row.column(v);
-      float x[N];
+      const int v = (int)~(uint32_t)from[i];
       Vec<T>::unpack(row.load(v), x);
+      c = row.column(v);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        key[j] = order_key(x[j], c + j);
-        if (key[j] >= bound && c + j >= 0 && c + j < row.V) mine |= 1u << j;
-      }
+      for (int j = 0; j < N; ++j) if (!(x[j] < least)) mine |= 1u << j;
+      if (!row.whole(v))
+        for (int j = 0; j < N; ++j) if (c + j < 0 || c + j >= row.V) mine &= ~(1u << j);
     }
-    append<N>(S.column_list(), &S.h.count, mine, key);
+    int2 at = reserve(&S.h.count, __popc(mine));
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (mine >> j & 1) S.column_list()[at.x++] = order_key(x[j], c + j);
   }
   shorten<NT, Vec<T>::SHIFT>(S);
 }
@@ -408,7 +415,9 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
   constexpr int N = Vec<T>::N, TILE = NT * U;
   const int tid = threadIdx.x;
   Sums a = no_sums();
-  bool more = false;
+  constexpr int ROUND = round_tiles(NT);
+  int in_round = 0;
+  float round_top = 0.f;
   for (int tile = begin; tile < end; tile += TILE) {
     const int first = tile + tid;
     uint4 raw[U];
@@ -464,9 +473,14 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
     a.s += s[0];
     if (ENTROPY) a.e += e[0] + e[1];
     if (TOP) {
-      const bool full = note<NT, U, Vec<T>::SHIFT>(*top_k, top, all, first, end, tile == begin);
-      more |= full;                                              // (looked at by all threads every ROOM tiles)
-      if (tile + TILE < end && ((tile - begin) / TILE + 1) % TopK::ROOM == 0) { make_room<NT, Vec<T>::SHIFT>(*top_k, more); more = false; }
+#pragma unroll
+      for (int u = 0; u < U; ++u) top_k->tops[(in_round * U + u) * NT + tid] = top[u];
+      round_top = in_round == 0 ? all : max_nan(round_top, all);
+      if (++in_round == ROUND || tile + TILE >= end) {
+        const int before = (in_round - 1) * TILE;
+        note<NT, U * ROUND, Vec<T>::SHIFT>(*top_k, round_top, first - before, end, tile - before == begin);
+        in_round = 0;
+      }
     }
   }
   return a;
@@ -494,11 +508,11 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
 // A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.
 template <typename T, int NT, int U, bool TOP>
 __global__ void __launch_bounds__(NT, NT == 32 ? TS_MB32 : TS_MB128 * 128 / NT)
-token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, double inv_t, int k, float* __restrict__ logprob,
+token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, float inv_t, int k, float* __restrict__ logprob,
                       float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids, float2* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
   extern __shared__ __align__(16) unsigned char dyn[];
-  TopK top(dyn, k, NT * U);                                      // (there is none without TOP)
+  TopK top(dyn, k, NT, NT * U * round_tiles(NT));                                     // (there is none without TOP)
   __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
   __shared__ Sums mine;
   const long long row_at = blockIdx.x / C;
@@ -569,9 +583,11 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   const int n = TOP ? top.h.keep : 0;
   const unsigned long long* list = TOP && top.h.from ? top.column_list() : top.kept;
   if (tid >= max(n, 1)) return;
-  const RowSum sum(a, c);
+  // ln of the sum relative to the largest logit: without the rounding of R
+  const float ln_s = logf(a.s) - LN2 * (careful(a) || !(fabsf(a.R) < FAR) ? 0.f : fmaf(a.top, c, -a.R));
+  const auto log_p = [&](float x) { return none ? -INFINITY : (x - a.top) * inv_t - ln_s; };
   if (tid == 0) {
-    logprob[row_at] = none ? -INFINITY : (float)sum.logprob(target, inv_t);
+    logprob[row_at] = log_p(target);
     // H = ln s - sum t 2^t / s, relative to the same R
     entropy[row_at] = none ? 0.f : LN2 * (log2f(a.s) - a.e / a.s);
     stats[row_at] = make_float2(a.top, none ? -INFINITY : log2f(a.s));
@@ -588,7 +604,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
     if (n & 1) before += list[n - 1] > key;
     if (before >= k) continue;
     top_ids[row_at * k + before] = (int)~(uint32_t)key;
-    top_lp[row_at * k + before] = none ? -INFINITY : (float)sum.logprob(key_value(key), inv_t);
+    top_lp[row_at * k + before] = log_p(key_value(key));
   }
 }
 
@@ -938,8 +954,8 @@ extern "C" int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t 
   do {                                                                                                                                                       \
     const int C = cluster_of(rows, pieces, NT * U);                                                                                                          \
     launch_cluster(top_k > 0 ? token_logprobs_kernel<T, NT, U, true> : token_logprobs_kernel<T, NT, U, false>, (long long)rows * C, NT,                      \
-                   top_k > 0 ? TopK::shared_bytes(top_k, NT, U) : 0, C, ST(stream), static_cast<const T*>(logits), (long long)ldl,                                         \
-                   tokens, (long long)ignore_index, log2_scale(temperature), 1. / temperature, (int)top_k, logprob, entropy, top_logprobs,    \
+                   top_k > 0 ? TopK::shared_bytes(top_k, NT, NT * U * round_tiles(NT)) : 0, C, ST(stream), static_cast<const T*>(logits), (long long)ldl,                                         \
+                   tokens, (long long)ignore_index, log2_scale(temperature), 1.f / temperature, (int)top_k, logprob, entropy, top_logprobs,    \
                    top_ids, reinterpret_cast<float2*>(row_stats), (int)V, C, status);                                                                        \
   } while (0)
   BY_TYPE(type, FORWARD, rows, pieces, CALL);
