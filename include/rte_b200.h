@@ -301,7 +301,8 @@ int rte_ce_gradient(const void* logits, int32_t f32, int32_t ldl, const int64_t*
                     const float* lse, void* dlogits, int32_t rows, int32_t V, int32_t* status, rte_stream_t stream);
 /* ------------------------------------------------ scores of tokens under rows of logits (no counterpart in the reference's table)
  * logits [rows, V] of `type`, row stride ldl in elements (any, 0 too); V, top_k and k as stated, lists of at most RTE_TOKEN_LIST_MAX.
- * Everything is taken of softmax(logits / temperature); -inf has probability zero, NaN or +inf make a row's results NaN.
+ * Everything is taken of softmax(logits / temperature), temperature in 1e-6 .. 1e6; -inf has probability zero, NaN or +inf make a row's
+ * results NaN.
  * rte_token_logprobs_fwd: logprob f32 [rows] of tokens[row], entropy f32 [rows], the top_k largest as top_logprobs f32 / top_ids
  *   int64 [rows, top_k] in descending order (equal logits: lower column first; NaN above all).  A row whose token is ignore_index (or
  *   out of range, which sets status) is not read: zeros, ids -1.  A row of nothing but -inf: log probabilities -inf, entropy 0.

@@ -28,13 +28,24 @@ constexpr int TS_MAX_LIST = RTE_TOKEN_LIST_MAX;
 constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.44269504088896340736, LN2_D = 0.693147180559945309417;
-constexpr float FAR = 1e36f;                   // exponents (in powers of two) beyond this are formed the careful way
+constexpr float FAR = 1e36f, LOW = -1e30f;     // exponents (in powers of two) and logits beyond these are taken the careful way
+constexpr float MIN_T = 1e-6f, MAX_T = 1e6f;   // temperatures: LOW is then far from all ordinary logits and within fp32 after scaling
 
 __device__ __forceinline__ float exp2_fast(float t) {            // two units in the last place, 0 below -126
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
+
+// Two fp32 values in one register pair, one instruction for both.
+struct Two {
+  unsigned long long v;
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ float lo() const { return __uint_as_float((uint32_t)v); }
+  __device__ __forceinline__ float hi() const { return __uint_as_float((uint32_t)(v >> 32)); }
+};
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v)); return c; }
+__device__ __forceinline__ Two add2(Two a, Two b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
 
 __device__ __forceinline__ float max_nan(float a, float b) {     // NaN where either is
   float r;
@@ -43,7 +54,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {     // NaN where ei
 }
 
 // ---------------------------------------------------------------- 16 bytes of a row
-template <typename T> struct Vec;              // N values; max: NaN where one of them is
+template <typename T> struct Vec;              // N values; max: NaN where one of them is; unpack_low: at least LOW
 template <> struct Vec<float> {
   static constexpr int SHIFT = 0;                       // low bits that a value's key does not use
   static constexpr int N = 4;
@@ -56,6 +67,11 @@ template <> struct Vec<float> {
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+  static __device__ __forceinline__ void unpack_low(const uint4& r, float (&x)[4]) {
+    unpack(r, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = max_nan(x[i], LOW);
   }
   static __device__ __forceinline__ float to_f(float v) { return v; }
   static __device__ __forceinline__ float from_f(float v) { return v; }
@@ -76,6 +92,13 @@ template <> struct Vec<__nv_bfloat16> {
   }
   static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
     return make_uint4(rte::pack_bf16x2(x[0], x[1]), rte::pack_bf16x2(x[2], x[3]), rte::pack_bf16x2(x[4], x[5]), rte::pack_bf16x2(x[6], x[7]));
+  }
+  static __device__ __forceinline__ void unpack_low(const uint4& r, float (&x)[8]) {
+    const __nv_bfloat162 low = __float2bfloat162_rn(LOW);
+    uint4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162*>(&q)[i] = __hmax2_nan(reinterpret_cast<const __nv_bfloat162*>(&r)[i], low);
+    unpack(q, x);
   }
   static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
@@ -100,6 +123,11 @@ template <> struct Vec<__half> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
     return r;
+  }
+  static __device__ __forceinline__ void unpack_low(const uint4& r, float (&x)[8]) {
+    unpack(r, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = max_nan(x[i], LOW);
   }
   static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
@@ -128,12 +156,14 @@ struct Row {
 };
 
 // ---------------------------------------------------------------- sums of exponentials
-// Exponents are kept in powers of two relative to R = max * c, c = log2(e) / T: t = x c - R in one fused step, whose rounded R shifts
-// every t of a row alike and is taken out again at the end.  R >= -FAR: all logits at the type's lowest value (or -inf) add nothing
-// then.  A row whose own R is beyond FAR (the type's ends at small temperatures, rows of nothing but lowest values) is summed again
-// relative to its maximum, t = (x - max) c.
+// Exponents are kept in powers of two relative to R = top * c, top the largest logit, c = log2(e) / T: t = x c - R in one fused step,
+// whose rounded R shifts every t of a row alike and is taken out again at the end.  Logits below LOW count as LOW (what is masked with
+// -inf or the type's lowest value: 2^t is 0, and t is finite, so that t 2^t is 0 too).  A row whose largest logit is itself
+// down there, or whose R is beyond FAR, is summed again, t = (x - top) c; a row of nothing but -inf has the sum 0.
 struct Sums { float top, R, s, e; };           // largest logit, reference, sum of 2^t, sum of t 2^t
-__device__ __forceinline__ Sums no_sums() { return {-INFINITY, -FAR, 0.f, 0.f}; }
+__device__ __forceinline__ float reference(float top, float c) { return fmaxf(top, LOW) * c; }
+__device__ __forceinline__ bool far(float top, float c) { return top <= 0.1f * LOW || !(fabsf(top * c) < FAR); }
+__device__ __forceinline__ Sums no_sums(float c) { return {-INFINITY, LOW * c, 0.f, 0.f}; }
 __device__ __forceinline__ void move_to(Sums& a, float R) {      // the same sums relative to R >= a.R
   const float d = a.R - R, f = exp2_fast(d);
   a.e = f * (a.e + d * a.s);
@@ -143,7 +173,7 @@ __device__ __forceinline__ void move_to(Sums& a, float R) {      // the same sum
 __device__ __forceinline__ float weighted(float t) { return fmaxf(t, -1e4f); }       // (t 2^t is 0 where t = -inf)
 
 template <int NT>
-__device__ __forceinline__ Sums block_sums(Sums a, Sums* red) {  // red: NT / 32 of them in shared memory; every thread gets the result
+__device__ __forceinline__ Sums block_sums(Sums a, float c, Sums* red) {  // red: NT / 32 of them in shared memory; every thread gets the result
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -152,7 +182,7 @@ __device__ __forceinline__ Sums block_sums(Sums a, Sums* red) {  // red: NT / 32
       __syncthreads();
       if (lane == 0) red[warp] = a;
       __syncthreads();
-      a = lane < NT / 32 ? red[lane] : no_sums();
+      a = lane < NT / 32 ? red[lane] : no_sums(c);
     }
     move_to(a, rte::warp_max(a.R));
     a.top = rte::warp_max(a.top);
@@ -161,13 +191,13 @@ __device__ __forceinline__ Sums block_sums(Sums a, Sums* red) {  // red: NT / 32
   }
   return a;
 }
-__device__ __forceinline__ bool careful(const Sums& a) { return a.top != -INFINITY && fabsf(a.R) >= FAR; }
+__device__ __forceinline__ bool careful(const Sums& a, float c) { return a.top != -INFINITY && far(a.top, c); }
 
 // What a row's sums say, in 64 bits: they are single values, and losses are small differences of them.
 struct RowSum {
   double top, ln_s, shift;                     // ln of sum exp((x - top) / T); log2 of what the stored sum is too large by
   __device__ __forceinline__ RowSum(const Sums& a, float c) : top(a.top) {
-    shift = careful(a) || !(fabsf(a.R) < FAR) ? 0. : (double)a.top * c - a.R;
+    shift = far(a.top, c) ? 0. : (double)a.top * c - a.R;
     ln_s = log((double)a.s) - shift * LN2_D;
   }
 };
@@ -175,9 +205,9 @@ struct RowSum {
 // The exponent of a logit relative to the row's largest, as forward formed it; p = 2^(t - l2) with l2 as forward kept it.
 struct Exponent {
   float top, c, R;
-  bool far;
-  __device__ __forceinline__ Exponent(float top_, float c_) : top(top_), c(c_), R(fmaxf(top_ * c_, -FAR)) { far = !(fabsf(R) < FAR); }
-  __device__ __forceinline__ float operator()(float x) const { return far ? (x - top) * c : fmaf(x, c, -R); }
+  bool is_far;
+  __device__ __forceinline__ Exponent(float top_, float c_) : top(top_), c(c_), R(reference(top_, c_)), is_far(far(top_, c_)) {}
+  __device__ __forceinline__ float operator()(float x) const { return is_far ? (x - top) * c : fmaf(x, c, -R); }
 };
 
 // ---------------------------------------------------------------- the largest logits of a row
@@ -258,8 +288,13 @@ __device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int 
   lo = (__reduce_min_sync(0xffffffffu, lo) + 1) >> SHIFT;
   hi = (__reduce_max_sync(0xffffffffu, hi) >> SHIFT) + 1;            // (no key is ~0)
   int at_lo = n;
-  while (hi - lo > 1 && at_lo > k + slack) {
-    const uint32_t mid = lo + (hi - lo) / 2, bound = mid << SHIFT;
+  for (int probe = 0; hi - lo > 1 && at_lo > k + slack; ++probe) {
+    uint32_t mid = lo + (hi - lo) / 2;
+    if (probe < 6) {                                     // halfway between the values first: logits lie about a mean, their keys about zero
+      const uint32_t half = value_key(0.5f * key_value((unsigned long long)lo << (32 + SHIFT)) + 0.5f * key_value((unsigned long long)(hi - 1) << (32 + SHIFT))) >> SHIFT;
+      if (half > lo && half < hi) mid = half;
+    }
+    const uint32_t bound = mid << SHIFT;
     int c = 0;
 #pragma unroll
     for (int u = 0; u < HELD; ++u) c += held[u] >= bound;
@@ -414,7 +449,7 @@ template <typename T, int NT, int U, bool ENTROPY, bool TOP, bool OUTSIDE>
 __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, float c, TopK* top_k, const int* id, int ids, uint32_t* bits) {
   constexpr int N = Vec<T>::N, TILE = NT * U;
   const int tid = threadIdx.x;
-  Sums a = no_sums();
+  Sums a = no_sums(c);
   constexpr int ROUND = round_tiles(NT);
   int in_round = 0;
   float round_top = 0.f;
@@ -449,29 +484,28 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
     }
     float top[U], all = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) { top[u] = Vec<T>::max(raw[u]); all = TOP ? max_nan(all, top[u]) : fmaxf(all, top[u]); }
-    if (all > a.top) {
-      a.top = all;
-      const float R = fmaxf(a.R, all * c);
-      if (ENTROPY) move_to(a, R);
-      else { a.s *= exp2_fast(a.R - R); a.R = R; }
-    }
-    const float negR = -a.R;
-    float s[2] = {0.f, 0.f}, e[2] = {0.f, 0.f};
+    for (int u = 0; u < U; ++u) { top[u] = Vec<T>::max(raw[u]); all = max_nan(all, top[u]); }
+    if (all > a.top) a.top = all;
+    if (!(all <= 0.1f * LOW)) {                                  // (else nothing but masked logits, or a row that is summed again)
+      const float R = fmaxf(a.R, reference(a.top, c));
+      if (R > a.R) move_to(a, R);
+      const Two cc(c, c), negR(-a.R, -a.R);
+      Two s(0.f, 0.f), e(0.f, 0.f);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[N];
-      Vec<T>::unpack(raw[u], x);
+      for (int u = 0; u < U; ++u) {
+        float x[N];
+        if (ENTROPY) Vec<T>::unpack_low(raw[u], x);
+        else Vec<T>::unpack(raw[u], x);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float t = fmaf(x[i], c, negR), p = exp2_fast(t);
-        s[i & 1] += p;
-        if (ENTROPY) e[i & 1] = fmaf(p, weighted(t), e[i & 1]);
+        for (int i = 0; i < N; i += 2) {
+          const Two t = fma2(Two(x[i], x[i + 1]), cc, negR), p(exp2_fast(t.lo()), exp2_fast(t.hi()));
+          s = add2(s, p);
+          if (ENTROPY) e = fma2(p, t, e);
+        }
       }
+      a.s += s.lo() + s.hi();
+      if (ENTROPY) a.e += e.lo() + e.hi();
     }
-    s[0] += s[1];
-    a.s += s[0];
-    if (ENTROPY) a.e += e[0] + e[1];
     if (TOP) {
 #pragma unroll
       for (int u = 0; u < U; ++u) top_k->tops[(in_round * U + u) * NT + tid] = top[u];
@@ -499,8 +533,7 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
     e = fmaf(p, weighted(t), e);
   }
   Sums a = {top, 0.f, s, e};
-  a = block_sums<NT>(a, red);
-  a.R = copysignf(FAR, top);
+  a = block_sums<NT>(a, c, red);
   return a;
 }
 
@@ -531,7 +564,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   if (rank == 0 && tid == 0) target = row.at((int)tok);
   const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
   Sums a = stream<T, NT, U, true, TOP, false>(row, begin, end, c, &top, nullptr, 0, nullptr);
-  a = block_sums<NT>(a, red);
+  a = block_sums<NT>(a, c, red);
   if (TOP) {
     if (begin < end) columns<T, NT>(top, row);
     else if (tid == 0) { top.h.keep = 0; top.h.from = 0; top.h.bound = 0; }
@@ -540,7 +573,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
     cg::cluster_group cluster = cg::this_cluster();
     if (tid == 0) mine = a;
     cluster.sync();
-    a = no_sums();
+    a = no_sums(c);
     for (int r = 0; r < C; ++r) {
       Sums b = *cluster.map_shared_rank(&mine, r);
       const float R = fmaxf(a.R, b.R);
@@ -550,7 +583,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
       a.s += b.s;
       a.e += b.e;
     }
-    if (careful(a)) {                                            // (all CTAs of the cluster see the same sums)
+    if (careful(a, c)) {                                            // (all CTAs of the cluster see the same sums)
       const Sums b = sums_far<T, NT, false>(row, begin, end, a.top, c, nullptr, 0, red);
       cluster.sync();
       if (tid == 0) mine = b;
@@ -576,7 +609,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
       cluster.sync();
     }
     if (rank != 0) return;
-  } else if (careful(a)) {
+  } else if (careful(a, c)) {
     a = sums_far<T, NT, false>(row, begin, end, a.top, c, nullptr, 0, red);
   }
   const bool none = a.s == 0.f;                                  // nothing but -inf
@@ -584,7 +617,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   const unsigned long long* list = TOP && top.h.from ? top.column_list() : top.kept;
   if (tid >= max(n, 1)) return;
   // ln of the sum relative to the largest logit: without the rounding of R
-  const float ln_s = logf(a.s) - LN2 * (careful(a) || !(fabsf(a.R) < FAR) ? 0.f : fmaf(a.top, c, -a.R));
+  const float ln_s = logf(a.s) - LN2 * (far(a.top, c) ? 0.f : fmaf(a.top, c, -a.R));
   const auto log_p = [&](float x) { return none ? -INFINITY : (x - a.top) * inv_t - ln_s; };
   if (tid == 0) {
     logprob[row_at] = log_p(target);
@@ -667,12 +700,12 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   }
   const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
   Sums a = stream<T, NT, U, false, false, TAIL>(row, begin, end, c, nullptr, id, k, bits);
-  a = block_sums<NT>(a, red);
+  a = block_sums<NT>(a, c, red);
   if (C > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     if (tid == 0) mine = a;
     cluster.sync();
-    a = no_sums();
+    a = no_sums(c);
     for (int r = 0; r < C; ++r) {
       Sums b = *cluster.map_shared_rank(&mine, r);
       const float R = fmaxf(a.R, b.R);
@@ -681,7 +714,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
       a.top = fmaxf(a.top, b.top);
       a.s += b.s;
     }
-    if (careful(a)) {
+    if (careful(a, c)) {
       const Sums b = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
       cluster.sync();
       if (tid == 0) mine = b;
@@ -692,7 +725,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
     }
     cluster.sync();                                              // (the others leave)
     if (rank != 0) return;
-  } else if (careful(a)) {
+  } else if (careful(a, c)) {
     a = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
   }
   // in 64 bits from here: a few values per row, whose small differences are the loss
@@ -742,7 +775,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   loss[row_at] = float(L * temp * temp);
   // log2 of the sum relative to the rounded reference that backward forms again
   const Exponent ex((float)top, c);
-  const double l2 = ln_s * LOG2E + (ex.far ? 0. : top * c - ex.R);
+  const double l2 = ln_s * LOG2E + (ex.is_far ? 0. : top * c - ex.R);
   stats[row_at * 2] = make_float4((float)top, (float)l2, float(M - (r > 0 ? r * exp(-ln_out) : 0.)), none ? 0.f : (float)M);
   stats[row_at * 2 + 1] = make_float4(TAIL ? 0.f : tmax, (float)shift, 0.f, 0.f);
 }
@@ -932,7 +965,7 @@ int pieces_of(const void* x, int type, long long ld, int V) {
     else WHICH(float, rows, pieces, CALL);                                    \
   } while (0)
 
-bool temperature_ok(float t) { return t >= 1e-30f && t <= 1e30f; }
+bool temperature_ok(float t) { return t >= MIN_T && t <= MAX_T; }
 bool rows_ok(const void* x, int type, int64_t ldl, int64_t rows, int64_t V) {
   return x && (type == RTE_TYPE_BF16 || type == RTE_TYPE_F16 || type == RTE_TYPE_F32) && rows > 0 && V > 0 && V <= TS_MAX_V && ldl >= 0;
 }

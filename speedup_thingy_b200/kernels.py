@@ -210,8 +210,8 @@ def _check_scores(name: str, logits, temperature, *others) -> None:
         raise ValueError(f"{name}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
     if logits.ndim == 0 or not 1 <= logits.shape[-1] < 2 ** 31 - 256:
         raise ValueError(f"{name}: logits [..., V] with at least one column, got {tuple(logits.shape)}")
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"{name}: the temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{name}: the temperature must be in 1e-6..1e6, got {temperature}")
     if any(t.device != logits.device for t in others):
         raise ValueError(f"{name}: all tensors must be on {logits.device}")
 
