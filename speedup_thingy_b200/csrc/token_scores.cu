@@ -193,21 +193,16 @@ __device__ __forceinline__ Sums block_sums(Sums a, float c, Sums* red) {  // red
 }
 __device__ __forceinline__ bool careful(const Sums& a, float c) { return a.top != -INFINITY && far(a.top, c); }
 
-// What a row's sums say, in 64 bits: they are single values, and losses are small differences of them.
-struct RowSum {
-  double top, ln_s, shift;                     // ln of sum exp((x - top) / T); log2 of what the stored sum is too large by
-  __device__ __forceinline__ RowSum(const Sums& a, float c) : top(a.top) {
-    shift = far(a.top, c) ? 0. : (double)a.top * c - a.R;
-    ln_s = log((double)a.s) - shift * LN2_D;
-  }
-};
-
 // The exponent of a logit relative to the row's largest, as forward formed it; p = 2^(t - l2) with l2 as forward kept it.
-struct Exponent {
-  float top, c, R;
-  bool is_far;
-  __device__ __forceinline__ Exponent(float top_, float c_) : top(top_), c(c_), R(reference(top_, c_)), is_far(far(top_, c_)) {}
-  __device__ __forceinline__ float operator()(float x) const { return is_far ? (x - top) * c : fmaf(x, c, -R); }
+struct Near {
+  float c, R;
+  __device__ __forceinline__ Near(float top, float c_) : c(c_), R(reference(top, c_)) {}
+  __device__ __forceinline__ float operator()(float x) const { return fmaf(x, c, -R); }
+};
+struct Far {
+  float top, c;
+  __device__ __forceinline__ Far(float top_, float c_) : top(top_), c(c_) {}
+  __device__ __forceinline__ float operator()(float x) const { return (x - top) * c; }
 };
 
 // ---------------------------------------------------------------- the largest logits of a row
@@ -312,7 +307,8 @@ __device__ __noinline__ unsigned long long warp_bound64(const unsigned long long
   const int lane = threadIdx.x & 31;
   int reach;
   const uint32_t* values = reinterpret_cast<const uint32_t*>(keys) + 1;
-  const uint32_t value = n <= 128 ? warp_bound<SHIFT, 2, 4>(values, n, k, slack, &reach) : warp_bound<SHIFT, 2, 16>(values, n, k, slack, &reach);
+  const uint32_t value = n <= 128 ? warp_bound<SHIFT, 2, 4>(values, n, k, slack, &reach)
+                                  : n <= 256 ? warp_bound<SHIFT, 2, 8>(values, n, k, slack, &reach) : warp_bound<SHIFT, 2, 16>(values, n, k, slack, &reach);
   if (reach <= k + slack) return (unsigned long long)value << 32;
   int above = 0;                                         // many equal values at the end: the lowest of their columns
   uint32_t same = 0;                                     // (their key, with the bits that were not searched)
@@ -444,7 +440,8 @@ __device__ __forceinline__ void columns(TopK& S, const Row<T>& row) {
 }
 
 // ---------------------------------------------------------------- one pass over a row's pieces [begin, end)
-// OUTSIDE: the columns of `id` (-1: none) are left out; `bits`: a bit per column of a tile, in shared memory.
+// OUTSIDE: the columns of `id` (-1: none) are left out; `bits`: a bit per column of MAP_TILES tiles, in shared memory.
+constexpr int MAP_TILES = 8;
 template <typename T, int NT, int U, bool ENTROPY, bool TOP, bool OUTSIDE>
 __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, float c, TopK* top_k, const int* id, int ids, uint32_t* bits) {
   constexpr int N = Vec<T>::N, TILE = NT * U;
@@ -460,17 +457,21 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
     for (int u = 0; u < U; ++u)
       raw[u] = first + u * NT < end ? row.load(first + u * NT) : make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
     if (OUTSIDE) {
-      __syncthreads();
-      for (int i = tid; i < TILE * N / 32; i += NT) bits[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < ids; i += NT) {
-        const int at = id[i] + row.off - tile * N;               // (id -1 lies before every tile's first column or is masked by the test)
-        if (id[i] >= 0 && at >= 0 && at < TILE * N) atomicOr(&bits[at >> 5], 1u << (at & 31));
+      const int in_map = (tile - begin) % (TILE * MAP_TILES);
+      if (in_map == 0) {
+        sync<NT>();
+        for (int i = tid; i < TILE * MAP_TILES * N / 32; i += NT) bits[i] = 0;
+        sync<NT>();
+        for (int i = tid; i < ids; i += NT) {
+          const int at = id[i] + row.off - tile * N;
+          if (id[i] >= 0 && at >= 0 && at < TILE * MAP_TILES * N) atomicOr(&bits[at >> 5], 1u << (at & 31));
+        }
+        sync<NT>();
       }
-      __syncthreads();
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const uint32_t listed = bits[(u * NT + tid) * N / 32] >> ((u * NT + tid) * N % 32) & ((1u << N) - 1);
+        const int at = (in_map + u * NT + tid) * N;
+        const uint32_t listed = bits[at / 32] >> (at % 32) & ((1u << N) - 1);
         if (listed) {
           uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
 #pragma unroll
@@ -664,16 +665,16 @@ __device__ __forceinline__ float block_max_float(float v, float* red) {
   return v;
 }
 
-// stats of a row, eight floats: largest logit, log2 of the sum, coefficient of p outside the list, M (0: no gradient), the list's
-// max, ln of its sum
+// stats of a row, eight floats: for the columns outside the list (all, without TAIL) their largest logit, log2 of their sum and what
+// their share of it is multiplied by; M (0: no gradient); the list's max, ln of its sum; the row's largest logit, log2 of its sum
 template <typename T, int NT, int U, bool TAIL>
 __global__ void __launch_bounds__(NT)
 distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, double temp,
                     float* __restrict__ loss, float4* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
-  __shared__ int id[TS_MAX_LIST];
+  __shared__ __align__(16) int id[TS_MAX_LIST];
   __shared__ float listed[TS_MAX_LIST];                          // the student's logits on the list
-  __shared__ uint32_t bits[TAIL ? NT * U * Vec<T>::N / 32 : 1];
+  __shared__ uint32_t bits[TAIL ? NT * U * MAP_TILES * Vec<T>::N / 32 : 1];
   __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
   __shared__ double red_d[NT / 32 > 0 ? NT / 32 : 1];
   __shared__ float red_f[NT / 32 > 0 ? NT / 32 : 1];
@@ -730,83 +731,93 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   }
   // in 64 bits from here: a few values per row, whose small differences are the loss
   const double inv_t = 1. / temp;
-  const RowSum others(a, c);
-  double top = others.top, ln_s = others.ln_s, ln_out = 0;       // the row's; ln of the others' share of it
+  float top = a.top;                                             // the row's largest logit
+  const double shift = far(a.top, c) ? 0. : (double)a.top * c - reference(a.top, c);      // log2 of what a.s is too large by
+  double s = a.s * exp2(-shift), ln_factor = 0;                  // the row's sum relative to `top`; ln of what a.s is relative to less than it
   if (TAIL) {
     float m = -INFINITY;
     for (int i = tid; i < k; i += NT) if (id[i] >= 0) m = fmaxf(m, listed[i]);
     top = block_max_float<NT>(fmaxf(m, a.top), red_f);
-    double s = 0;
+    double l = 0;
     if (top != -INFINITY)
       for (int i = tid; i < k; i += NT) {
         bool again = id[i] < 0;                                  // a token that an earlier slot names too counts once
-        for (int j = 0; j < i; ++j) again |= id[j] == id[i];
-        if (!again) s += exp((listed[i] - top) * inv_t);
+        for (int j = 0; j < i; j += 4) {
+          const int4 v = *reinterpret_cast<const int4*>(id + j);
+          again |= v.x == id[i] || (j + 1 < i && v.y == id[i]) || (j + 2 < i && v.z == id[i]) || (j + 3 < i && v.w == id[i]);
+        }
+        if (!again) l += expf((float)((listed[i] - (double)top) * inv_t));
       }
-    s = block_sum_double<NT>(s, red_d);
-    const double ln_others = (others.top - top) * inv_t + others.ln_s;         // -inf: nothing outside the list
-    if (a.s != 0.f) s += exp(ln_others);
-    ln_s = log(s);
-    ln_out = ln_others - ln_s;
+    l = block_sum_double<NT>(l, red_d);
+    ln_factor = a.s == 0.f ? 0. : ((double)a.top - top) * inv_t;
+    s = l + s * exp(ln_factor);
   }
-  const bool none = top == -INFINITY && !(ln_s != ln_s);         // nothing but -inf
-  double shift = 0;
+  const double ln_s = log(s);
+  const bool none = top == -INFINITY && s == 0;                  // nothing but -inf
+  double t_shift = 0;
   if (!TAIL) {
     const float m = block_max_float<NT>(tmax, red_f);
-    double s = 0;
-    for (int i = tid; i < k; i += NT) if (id[i] >= 0) s += exp((double)t[i] - m);
-    s = block_sum_double<NT>(s, red_d);
+    double l = 0;
+    for (int i = tid; i < k; i += NT) if (id[i] >= 0) l += exp((double)t[i] - m);
+    l = block_sum_double<NT>(l, red_d);
     tmax = m;
-    shift = log(s);
+    t_shift = log(l);
   }
   double M = 0, L = 0;
   for (int i = tid; i < k; i += NT) {
     if (id[i] < 0) continue;
-    const double lq = TAIL ? (double)t[i] : (double)t[i] - tmax - shift, q = exp(lq);
+    const double lq = TAIL ? (double)t[i] : (double)t[i] - tmax - t_shift, q = exp(lq);
     M += q;
-    if (q != 0) L += q * (lq - (none ? -INFINITY : (listed[i] - top) * inv_t - ln_s));
+    if (q != 0) L += q * (lq - (none ? -INFINITY : (listed[i] - (double)top) * inv_t - ln_s));
   }
   M = block_sum_double<NT>(M, red_d);
   L = block_sum_double<NT>(L, red_d);
   if (tid != 0) return;
-  const double r = TAIL && a.s > 0.f && !none ? fmax(0., 1 - M) : 0.;
-  if (r > 0) L += r * (log(r) - ln_out);
-  M += r;
+  double P = 1;                                                  // the others' probability
+  if (TAIL) {
+    const double r = a.s > 0.f ? fmax(0., 1 - M) : 0., ln_out = ln_factor + log((double)a.s) - shift * LN2_D - ln_s;
+    P = exp(ln_out);
+    if (r > 0) L += r * (log(r) - ln_out);
+    M += r;
+    P = M * P - r;                                               // (what the others' gradient is in proportion to)
+  }
   loss[row_at] = float(L * temp * temp);
-  // log2 of the sum relative to the rounded reference that backward forms again
-  const Exponent ex((float)top, c);
-  const double l2 = ln_s * LOG2E + (ex.is_far ? 0. : top * c - ex.R);
-  stats[row_at * 2] = make_float4((float)top, (float)l2, float(M - (r > 0 ? r * exp(-ln_out) : 0.)), none ? 0.f : (float)M);
-  stats[row_at * 2 + 1] = make_float4(TAIL ? 0.f : tmax, (float)shift, 0.f, 0.f);
+  // 2^-l2 of a sum relative to the rounded reference that backward forms again: the others' among themselves, and the row's
+  const bool others = a.s != 0.f;
+  const double l2 = ln_s * LOG2E + (far(top, c) ? 0. : (double)top * c - reference(top, c));
+  stats[row_at * 2] = make_float4(others ? a.top : 0.f, others ? log2f(a.s) : 0.f, !others ? 0.f : TAIL ? (float)P : (float)M, none ? 0.f : (float)M);
+  stats[row_at * 2 + 1] = make_float4(TAIL ? 0.f : tmax, (float)t_shift, top, (float)l2);
 }
 
 // ---------------------------------------------------------------- backward
-// A CTA per NT * U pieces of a row: p from the row's saved maximum and sum, the same for all columns; then the listed columns again.
+// A CTA per NT * U pieces of a row: what all columns get first, from the row's saved maximum and sum; then its first warp writes the
+// listed columns again.
 template <typename T, int NT, int U>
 struct Slice {
-  Row<T> row, out;
-  int first, end;                                                // pieces
-  __device__ __forceinline__ Slice(const T* x, T* dx, int V, int part) : row(x, V), out(dx, V), first(part * NT * U + threadIdx.x), end(row.pieces) {}
+  Row<T> row;
+  T* dx;
+  bool even;                                                     // logits and gradient lie alike on 16 bytes
+  int first;                                                     // piece
+  __device__ __forceinline__ Slice(const T* x, T* dx_, int V, int part)
+      : row(x, V), dx(dx_), even(((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx_)) & 15) == 0), first(part * NT * U + threadIdx.x) {}
   __device__ __forceinline__ bool holds(long long column, int part) const {
     const long long v = (column + row.off) / Vec<T>::N - (long long)part * NT * U;
     return column >= 0 && column < row.V && v >= 0 && v < NT * U;
   }
   __device__ __forceinline__ void store(int v, const float (&y)[Vec<T>::N]) const {
-    T* dx = const_cast<T*>(out.x);
     const int c = row.column(v);
-    if (row.whole(v) && row.off == out.off) { *reinterpret_cast<uint4*>(dx + c) = Vec<T>::pack(y); return; }
+    if (even && row.whole(v)) { *reinterpret_cast<uint4*>(dx + c) = Vec<T>::pack(y); return; }
 #pragma unroll
     for (int i = 0; i < Vec<T>::N; ++i) if (c + i >= 0 && c + i < row.V) dx[c + i] = Vec<T>::from_f(y[i]);
   }
-  __device__ __forceinline__ void load(uint4 (&raw)[U]) const {
-#pragma unroll
-    for (int u = 0; u < U; ++u) if (first + u * NT < end) raw[u] = row.load(first + u * NT);
-  }
   template <typename F>
-  __device__ __forceinline__ void each(const uint4 (&raw)[U], F f) const {
+  __device__ __forceinline__ void each(F f) const {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) if (first + u * NT < row.pieces) raw[u] = row.load(first + u * NT);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (first + u * NT >= end) break;
+      if (first + u * NT >= row.pieces) break;
       float x[Vec<T>::N];
       Vec<T>::unpack(raw[u], x);
 #pragma unroll
@@ -816,65 +827,50 @@ struct Slice {
   }
   __device__ __forceinline__ void zero() const {
     const float y[Vec<T>::N] = {};
-    for (int u = 0; u < U; ++u) if (first + u * NT < end) store(first + u * NT, y);
+    for (int u = 0; u < U; ++u) if (first + u * NT < row.pieces) store(first + u * NT, y);
   }
 };
 
 template <typename T, int NT, int U>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, NT == 32 ? 24 : 2048 / NT)
 token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, float c, float inv_t, int k, const int64_t* __restrict__ top_ids,
                           const float2* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ g_lp, const float* __restrict__ g_h,
                           const float* __restrict__ g_top, T* __restrict__ dlogits, int V, int parts) {
   rte::after_previous_grid();
-  __shared__ float red[NT / 32 > 0 ? NT / 32 : 1];
-  __shared__ int on_list;
   const long long row_at = blockIdx.x / parts, tok = tokens[row_at];
   const int part = blockIdx.x % parts, tid = threadIdx.x;
   const float2 st = stats[row_at];
   const Slice<T, NT, U> slice(logits + row_at * ld, dlogits + row_at * V, V, part);
   if (tok < 0 || tok >= V || st.y == -INFINITY) return slice.zero();
-  uint4 raw[U];                                                  // (requested ahead of what depends on other loads)
-  slice.load(raw);
   const float g = g_lp ? g_lp[row_at] : 0.f, gh = g_h ? g_h[row_at] : 0.f;
-  float all = g;
-  if (!g_top) k = 0;
-  if (k > 0) {
-    float s = 0.f;
-    for (int i = tid; i < k; i += NT) s += g_top[row_at * k + i];
-    s = rte::warp_sum(s);
-    if (tid == 0) on_list = 0;
-    if (NT > 32) {
-      if ((tid & 31) == 0) red[tid >> 5] = s;
-      __syncthreads();
-      s = 0.f;
-      for (int w = 0; w < NT / 32; ++w) s += red[w];
-    } else {
-      __syncwarp();
-    }
-    all += s;
-  }
+  float all = 0.f;
+  for (int i = tid & 31; g_top && i < k; i += 32) all += g_top[row_at * k + i];        // (every warp for itself)
+  all = g + rte::warp_sum(all);
   // dx = -p (all + gh (ln p + H)) / T
-  const Exponent ex(st.x, c);
   const float a = -(all + gh * entropy[row_at]) * inv_t, b = -gh * LN2 * inv_t;
-  const auto base = [&](float x) {
-    const float l = ex(x) - st.y;
-    return exp2_fast(l) * fmaf(b, weighted(l), a);
+  const auto write = [&](auto exponent) {
+    const auto base = [&](float x) {
+      const float l = exponent(x) - st.y;
+      return exp2_fast(l) * fmaf(b, weighted(l), a);
+    };
+    slice.each(base);
+    sync<NT>();
+    if (tid >= 32) return;
+    bool target_done = !g_lp || !slice.holds(tok, part);
+    for (int i = tid; g_top && i - tid < k; i += 32) {
+      const long long j = i < k ? top_ids[row_at * k + i] : -1;
+      const bool target = j == tok, mine = slice.holds(j, part);
+      if (mine) dlogits[row_at * V + j] = Vec<T>::from_f(base(slice.row.at((int)j)) + (g_top[row_at * k + i] + (target ? g : 0.f)) * inv_t);
+      target_done |= __any_sync(0xffffffffu, target && mine);
+    }
+    if (!target_done && tid == 0) dlogits[row_at * V + tok] = Vec<T>::from_f(base(slice.row.at((int)tok)) + g * inv_t);
   };
-  slice.each(raw, base);
-  __syncthreads();
-  for (int i = tid; i < k; i += NT) {
-    const long long j = top_ids[row_at * k + i];
-    if (!slice.holds(j, part)) continue;
-    const bool target = j == tok;
-    if (target) on_list = 1;
-    dlogits[row_at * V + j] = Vec<T>::from_f(base(slice.row.at((int)j)) + (g_top[row_at * k + i] + (target ? g : 0.f)) * inv_t);
-  }
-  if (k > 0) __syncthreads();
-  if (tid == 0 && g_lp && slice.holds(tok, part) && !(k > 0 && on_list)) dlogits[row_at * V + tok] = Vec<T>::from_f(base(slice.row.at((int)tok)) + g * inv_t);
+  if (far(st.x, c)) write(Far(st.x, c));
+  else write(Near(st.x, c));
 }
 
 template <typename T, int NT, int U>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, NT == 32 ? 24 : 2048 / NT)
 distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, float temp,
                         const float4* __restrict__ stats, const float* __restrict__ dloss, T* __restrict__ dlogits, int V, int parts) {
   rte::after_previous_grid();
@@ -882,27 +878,43 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
   __shared__ float q[TS_MAX_LIST];
   const long long row_at = blockIdx.x / parts;
   const int part = blockIdx.x % parts, tid = threadIdx.x;
-  const float4 st = stats[row_at * 2], list = stats[row_at * 2 + 1];
+  const float4 st = stats[row_at * 2];
   const Slice<T, NT, U> slice(logits + row_at * ld, dlogits + row_at * V, V, part);
   if (st.w == 0.f) return slice.zero();
-  uint4 raw[U];
-  slice.load(raw);
-  for (int i = tid; i < k; i += NT) {
-    const long long j = ids[row_at * k + i];
-    id[i] = slice.holds(j, part) ? (int)j : -1;
-    if (id[i] >= 0) q[i] = expf(teacher[row_at * k + i] - list.x - list.y);
+  const float scale = dloss[row_at] * temp;
+  {
+    const float outside = scale * st.z;
+    if (far(st.x, c)) { const Far t(st.x, c); slice.each([&](float x) { return exp2_fast(t(x) - st.y) * outside; }); }
+    else { const Near t(st.x, c); slice.each([&](float x) { return exp2_fast(t(x) - st.y) * outside; }); }
   }
-  const Exponent ex(st.x, c);
-  const float scale = dloss[row_at] * temp, outside = scale * st.z, inside = scale * st.w;
-  slice.each(raw, [&](float x) { return exp2_fast(ex(x) - st.y) * outside; });
-  __syncthreads();
-  for (int i = tid; i < k; i += NT) {
-    if (id[i] < 0) continue;
+  sync<NT>();
+  if (tid >= 32) return;
+  const float4 list = stats[row_at * 2 + 1];
+  const float inside = scale * st.w;
+  const bool is_far = far(list.z, c);
+  const Far from(list.z, c);
+  const Near near(list.z, c);
+  int n = 0;                                                     // the slots that name a column of this slice, in their order
+  for (int i = tid; i - tid < k; i += 32) {
+    const long long j = i < k ? ids[row_at * k + i] : -1;
+    const bool mine = slice.holds(j, part);
+    const uint32_t who = __ballot_sync(0xffffffffu, mine);
+    if (mine) {
+      const int at = n + __popc(who & ((1u << tid) - 1));
+      id[at] = (int)j;
+      q[at] = expf(teacher[row_at * k + i] - list.x - list.y);
+    }
+    n += __popc(who);
+  }
+  __syncwarp();
+  for (int i = tid; i < n; i += 32) {
     bool again = false;                                          // a token named by several slots: the first of them writes
     float sum = 0.f;
-    for (int j = 0; j < k; ++j)
+    for (int j = 0; j < n; ++j)
       if (id[j] == id[i]) { again |= j < i; sum += q[j]; }
-    if (!again) dlogits[row_at * V + id[i]] = Vec<T>::from_f(exp2_fast(ex(slice.row.at(id[i])) - st.y) * inside - scale * sum);
+    if (again) continue;
+    const float x = slice.row.at(id[i]);
+    dlogits[row_at * V + id[i]] = Vec<T>::from_f(exp2_fast((is_far ? from(x) : near(x)) - list.w) * inside - scale * sum);
   }
 }
 

@@ -293,12 +293,13 @@ def distill64(x, teacher, ids, T, tail):
     M = q.sum(-1)
     dz = M[..., None] * p - qd
     if tail:
-        out = p.masked_fill(member, 0.0)
-        P = out.sum(-1)
-        r = (1 - M).clamp(min=0.0).masked_fill(P == 0, 0.0)
-        safe = P.masked_fill(P == 0, 1.0)
-        loss = loss + torch.where(r > 0, r * (r.clamp(min=1e-300).log() - safe.log()), torch.zeros_like(r))
-        dz = dz + r[..., None] * (p - out / safe[..., None])
+        # (in logarithms: e^-745 is the smallest number of 64 bits)
+        outside = logp.masked_fill(member, -INF)
+        lnP = torch.logsumexp(outside, -1)
+        r = (1 - M).clamp(min=0.0).masked_fill(lnP == -INF, 0.0)
+        lnP = lnP.masked_fill(lnP == -INF, 0.0)
+        loss = loss + torch.where(r > 0, r * (r.clamp(min=1e-300).log() - lnP), torch.zeros_like(r))
+        dz = dz + r[..., None] * (p - (outside - lnP[..., None]).exp())
     loss = (T * T * loss).masked_fill(none, 0.0)
     dz = (T * dz).masked_fill((none | empty)[..., None], 0.0)
     return loss, dz, dict(none=none, p=p, q=q, qd=qd, logp=logp, lp=lp, M=M)
@@ -377,6 +378,21 @@ def test_distillation_lists_in_every_state(V, tail, dtype):
     t[:] = -INF
     none = check_distill(x, t, ids, 1.0, tail)
     assert tail or not none.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 3000, 40001])
+def test_the_rest_of_the_vocabulary_far_below_the_list(V, dtype):
+    """Its probability is below fp32's range, its logarithm and the gradient that it takes are ordinary numbers."""
+    x = made(4, V, dtype)
+    t, ids = a_teacher(x, 5, 1.0)
+    t = t - t.logsumexp(-1, keepdim=True) - 0.7
+    for row, height in enumerate((90.0, 300.0, 900.0, 20000.0)):
+        x[row, ids[row]] = height
+    x[3, : V // 2] = -INF
+    x[3, ids[3]] = 20000.0
+    loss = check_distill(x, t, ids, 1.0, True)
+    assert loss.isfinite().all() and (loss[1:] > 100).all()
 
 
 def test_a_listed_id_outside_the_vocabulary_is_noted():
