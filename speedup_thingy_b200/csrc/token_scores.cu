@@ -19,12 +19,9 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-#ifndef TS_MB32
-#define TS_MB32 24
-#define TS_MB128 10
-#define TS_R128 2
-#endif
 constexpr int TS_MAX_LIST = RTE_TOKEN_LIST_MAX;
+// Forward's CTAs on an SM: 24 to 32 warps are in flight, a thread has 85, 48 or 64 registers.
+__host__ __device__ constexpr int min_ctas(int nt) { return nt == 32 ? 24 : nt == 128 ? 10 : 4; }
 constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.44269504088896340736, LN2_D = 0.693147180559945309417;
@@ -238,8 +235,8 @@ struct TopK {                                            // in shared memory, si
         top(reinterpret_cast<uint32_t*>(piece + cap_of(k_, round))), k(k_), cap(cap_of(k_, round)), tops(reinterpret_cast<float*>(top + nt)) {}
   __device__ __forceinline__ unsigned long long* column_list() const { return piece + most(k); }
 };
-// Tiles whose pieces' maxima are kept before they are looked through: 512 pieces or 2048.
-__host__ __device__ constexpr int round_tiles(int nt) { return nt == 256 ? 2 : nt == 128 ? TS_R128 : 4; }
+// Tiles whose pieces' maxima are kept before they are looked through: 512, 1024 and 2048 pieces.
+__host__ __device__ constexpr int round_tiles(int nt) { return nt == 256 ? 1 : nt == 128 ? 2 : 4; }
 
 template <int NT> __device__ __forceinline__ void sync() { if (NT == 32) __syncwarp(); else __syncthreads(); }
 template <int NT> __device__ __forceinline__ int sync_or(int v) { return NT == 32 ? __any_sync(0xffffffffu, v) : __syncthreads_or(v); }
@@ -541,7 +538,7 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
 // ---------------------------------------------------------------- forward
 // A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.
 template <typename T, int NT, int U, bool TOP>
-__global__ void __launch_bounds__(NT, NT == 32 ? TS_MB32 : TS_MB128 * 128 / NT)
+__global__ void __launch_bounds__(NT, min_ctas(NT))
 token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, float inv_t, int k, float* __restrict__ logprob,
                       float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids, float2* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
@@ -668,7 +665,7 @@ __device__ __forceinline__ float block_max_float(float v, float* red) {
 // stats of a row, eight floats: for the columns outside the list (all, without TAIL) their largest logit, log2 of their sum and what
 // their share of it is multiplied by; M (0: no gradient); the list's max, ln of its sum; the row's largest logit, log2 of its sum
 template <typename T, int NT, int U, bool TAIL>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, min_ctas(NT))
 distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, double temp,
                     float* __restrict__ loss, float4* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
@@ -951,24 +948,22 @@ int pieces_of(const void* x, int type, long long ld, int V) {
 }
 
 // A row of at most one tile of 32 or 128 threads is one CTA of them; longer ones are walked by 256.
-#ifndef TS_FEW
-#define TS_FEW 2960
-#define TS_NB 128
-#define TS_WIDE 296
-#endif
-// Forward: a row of up to four tiles of a warp is that warp's where there are rows enough, others are walked by 128 threads.
-#define FORWARD(T, rows, pieces, CALL)                        \
-  do {                                                        \
-    if (pieces <= 128 || (pieces <= 512 && rows >= TS_FEW)) CALL(T, 32, 4); \
-    else if (rows >= TS_WIDE || pieces <= 512) CALL(T, 128, 4);                                     \
-    else CALL(T, 256, 4);                                     \
+// Forward, who walks a row.  Many short rows: a warp each (us, 8192 x 2048 bf16, warp | 128 threads: 11.0 | 20, with 32 alternatives 39 | 60;
+// 256 rows of it: 6.2 | 4.8).  Many long ones: 128 threads (8192 x 32768 bf16, warp | 128 | 256 | 512: 119 | 97 | 105 | 151).  Few long ones,
+// where latency counts: 256 threads, eight loads each (1 x 50257 with 20 alternatives, 128 x 4 | 256 x 4 | 256 x 8: 12.8 | 10.7 | 9.2).
+constexpr int MANY_SHORT = 20 * 148, MANY_LONG = 2 * 148;
+#define FORWARD(T, rows, pieces, CALL)                                              \
+  do {                                                                              \
+    if (pieces <= 128 || (pieces <= 512 && rows >= MANY_SHORT)) CALL(T, 32, 4);     \
+    else if (pieces <= 512 || rows >= MANY_LONG) CALL(T, 128, 4);                   \
+    else CALL(T, 256, 8);                                                           \
   } while (0)
-// Backward: as many threads as four pieces each cover the row with, up to 256.
+// Backward: CTAs of a warp for rows that it covers, of 128 threads for others, all 2048 of an SM (8192 x 32768 bf16, 128 | 256 threads:
+// 163 | 174; 8192 x 2048, warp | 128: 17.9 | 13.7).
 #define BACKWARD(T, rows, pieces, CALL)     \
   do {                                      \
     if (pieces <= 128) CALL(T, 32, 4);      \
-    else if (pieces <= 512) CALL(T, 128, 4); \
-    else CALL(T, TS_NB, 4);                   \
+    else CALL(T, 128, 4);                   \
   } while (0)
 #define BY_TYPE(type, WHICH, rows, pieces, CALL)                              \
   do {                                                                        \
