@@ -3,11 +3,13 @@
 //   y_t = scale * w[id_t],     dw_v = scale * sum over { t : id_t = v } of dy_t,  in fp32, rounded once
 //
 // The gradient's addends meet in the order of the tokens, whatever the launch: the token positions are sorted by (id, position), a
-// thread adds its columns of RANGE consecutive sorted rows, what a range adds for an id that reaches beyond it goes to a partial, and
-// the range in which such an id begins adds the partials in order.  No atomics; rows that no token names are zeros.
+// thread adds its columns of a range of consecutive sorted rows, what a range adds for an id that reaches beyond it goes to a
+// partial, and those of one id are added in order.  No atomics on values; rows that no token names are zeros.
 //
-// The sort counts: the place of token i in its chunk of CHUNK tokens is the number of tokens j of the chunk with
-// (id_j, j) < (id_i, i); a second launch adds, for every other chunk, how many of its ids come before, by binary search.
+// The sort: up to SORT_RANK tokens each counts the tokens that come before it.  More take a pass per digit of the id (two digits of up to 10
+// bits for tables of up to 2^20 rows), each stable: a CTA's tokens are counted by digit, and a token's place is the number of
+// tokens with a smaller digit, those with its own in CTAs before, in warps before, and in its warp before it.  A pass leaves the next digit's
+// counts behind, so that a sort of two digits is three launches.
 
 #include <cuda_fp16.h>
 
@@ -15,7 +17,10 @@
 
 namespace {
 
-constexpr int EO_CHUNK = 4096, EO_RANGE = 32, EO_LANES = 8;          // tokens a chunk, sorted rows a range, threads that count for one token
+constexpr int SORT_RANK = 2048, SORT_LANES = 8;                      // tokens that are ranked by counting, threads that count for one
+constexpr int SORT_THREADS = 256, SORT_TILE = 2048, SORT_CTAS = 296; // tokens a CTA places at a time; CTAs at most
+constexpr int SORT_BITS = 10;                                        // of a digit, at most
+constexpr int ROWS_AHEAD = 8, MAX_RANGE = 64;                        // rows a thread has in flight; sorted rows of a range at most
 
 // `BYTES` of a row at a time, as fp32
 template <typename T, int BYTES> struct Piece {
@@ -48,43 +53,78 @@ __device__ __forceinline__ typename Raw<T, BYTES>::type pack(const Piece<T, BYTE
   return raw;
 }
 
-// A thread per piece of a row.
+// 128 threads as groups of `tpr`, a power of two, a thread per piece of a row and further ones where a row has more than 128.
+int threads_per_row(int pieces) {
+  int t = 1;
+  while (t < pieces && t < 128) t *= 2;
+  return t;
+}
+
+// A group takes TOKENS_AHEAD tokens at a time.
+constexpr int TOKENS_AHEAD = 4;
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(256)
-embedding_fwd_kernel(const int64_t* __restrict__ ids, long long n, const T* __restrict__ table, int V, int pieces, float scale, T* __restrict__ out, int* status) {
+__global__ void __launch_bounds__(128)
+embedding_fwd_kernel(const int64_t* __restrict__ ids, long long n, const T* __restrict__ table, int V, int pieces, int tpr, float scale, T* __restrict__ out, int* status) {
   rte::after_previous_grid();
   using R = typename Raw<T, BYTES>::type;
   const R* w = reinterpret_cast<const R*>(table);
   R* y = reinterpret_cast<R*>(out);
-  const long long total = n * pieces;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const long long t = i / pieces, id = ids[t];
-    const int c = int(i - t * pieces);
-    if (id < 0 || id >= V) {
-      if (status && c == 0) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
-      y[i] = R{};
-    } else {
-      y[i] = pack<T, BYTES>(unpack<T, BYTES>(w[id * pieces + c]), scale);
+  const int lane = threadIdx.x % tpr, groups = 128 / tpr;
+  for (long long t = ((long long)blockIdx.x * groups + threadIdx.x / tpr) * TOKENS_AHEAD; t < n; t += (long long)gridDim.x * groups * TOKENS_AHEAD) {
+    long long id[TOKENS_AHEAD];
+#pragma unroll
+    for (int u = 0; u < TOKENS_AHEAD; ++u) {
+      id[u] = t + u < n ? ids[t + u] : 0;
+      if (id[u] < 0 || id[u] >= V) {
+        if (status && lane == 0 && blockIdx.y == 0) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
+        id[u] = -1;
+      }
+    }
+    for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) {
+      R r[TOKENS_AHEAD];
+#pragma unroll
+      for (int u = 0; u < TOKENS_AHEAD; ++u) r[u] = id[u] >= 0 ? w[id[u] * pieces + c] : R{};
+#pragma unroll
+      for (int u = 0; u < TOKENS_AHEAD; ++u)
+        if (t + u < n) y[(t + u) * pieces + c] = pack<T, BYTES>(unpack<T, BYTES>(r[u]), scale);
     }
   }
 }
 
+// ---------------------------------------------------------------- the gradient's workspace
+struct Digits { int passes, bits; };           // of ids 0 .. V (V: takes no gradient)
+Digits digits_of(int V) {
+  int b = 1;
+  while (b < 31 && V >> b) ++b;
+  const int passes = b <= SORT_BITS ? 1 : (b + SORT_BITS - 1) / SORT_BITS;
+  return {passes, (b + passes - 1) / passes};
+}
 struct EoScratch {
-  int *chunk_id, *chunk_tok;      // [n]: every chunk sorted
-  int *id, *tok;                  // [n]: all sorted (the same two where there is one chunk)
-  float* part;                    // [ranges][2][d]: what a range adds for an id that began before it | that goes on after it
+  int *id, *tok;                // [n]: sorted
+  int *id2, *tok2;              // [n]: between passes
+  int* hist;                    // [passes][sort CTAs][1 << bits]
+  int *joins, *join_count;      // ranges whose last id goes on behind them and did not begin before them
+  float* part;                  // [ranges][2][d]: what a range adds for an id that began before it | that goes on behind it
 };
-inline size_t eo_layout(char* at, long long n, int d, EoScratch* s) {
+int sort_span(long long n) { return (int)rte::ceil_div64(rte::ceil_div64(n, SORT_TILE), SORT_CTAS) * SORT_TILE; }      // tokens of a sort CTA
+int range_of(long long n) { return n >= 32768 ? MAX_RANGE : 32; }
+size_t eo_layout(char* at, long long n, int d, EoScratch* s) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  const size_t list = up((size_t)n * 4), lists = n > EO_CHUNK ? 4 : 2, part = up((size_t)rte::ceil_div64(n, EO_RANGE) * 2 * d * 4);
+  const size_t list = up((size_t)n * 4), ranges = (size_t)rte::ceil_div64(n, range_of(n));
+  // (three digits of 10 bits and one more pass: what a table of any size takes)
+  const size_t hist = n > SORT_RANK ? up((size_t)4 * rte::ceil_div64(n, sort_span(n)) * (1 << SORT_BITS) * 4) : 0;
+  const size_t lists = n > SORT_RANK ? 4 : 2;
   if (s) {
-    s->chunk_id = reinterpret_cast<int*>(at);
-    s->chunk_tok = reinterpret_cast<int*>(at + list);
-    s->id = reinterpret_cast<int*>(at + (lists - 2) * list);
-    s->tok = reinterpret_cast<int*>(at + (lists - 1) * list);
-    s->part = reinterpret_cast<float*>(at + lists * list);
+    s->id = reinterpret_cast<int*>(at);
+    s->tok = reinterpret_cast<int*>(at + list);
+    s->id2 = reinterpret_cast<int*>(at + 2 * list);
+    s->tok2 = reinterpret_cast<int*>(at + 3 * list);
+    s->hist = reinterpret_cast<int*>(at + lists * list);
+    s->join_count = reinterpret_cast<int*>(at + lists * list + hist);
+    s->joins = s->join_count + 64;
+    s->part = reinterpret_cast<float*>(at + lists * list + hist + 256 + up(ranges * 4));
   }
-  return lists * list + part;
+  return lists * list + hist + 256 + up(ranges * 4) + up(ranges * 2 * d * 4);
 }
 
 // Ids that take no gradient (padding, out of range) count as V: behind all others.
@@ -94,32 +134,156 @@ __device__ __forceinline__ int eo_id(long long v, int V, long long padding, int*
   return V;
 }
 
-// blockIdx.y: chunk; a CTA places 256 / EO_LANES of its tokens, EO_LANES threads counting for each.
-__global__ void __launch_bounds__(256)
-embedding_rank_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int* status) {
+// Zeros, by the CTAs that a sort's launch has beside those that sort: a sort leaves most of the memory's time to them.
+struct Fill { char* at; long long bytes; };
+__device__ __forceinline__ void fill(const Fill& f, int cta, int ctas) {
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const long long head = min(f.bytes, (long long)(-reinterpret_cast<uintptr_t>(f.at) & 15)), body = (f.bytes - head) / 16;
+  uint4* q = reinterpret_cast<uint4*>(f.at + head);
+  for (long long i = (long long)cta * nt + tid; i < body; i += (long long)ctas * nt) q[i] = make_uint4(0, 0, 0, 0);
+  if (cta == 0) {
+    for (long long i = tid; i < head; i += nt) f.at[i] = 0;
+    for (long long i = head + body * 16 + tid; i < f.bytes; i += nt) f.at[i] = 0;
+  }
+}
+
+// ---------------------------------------------------------------- sort
+// Up to SORT_RANK tokens: a CTA places SORT_THREADS / SORT_LANES of them.
+__global__ void __launch_bounds__(SORT_THREADS)
+embedding_rank_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, Fill f, int ctas, int* status) {
   rte::after_previous_grid();
-  __shared__ __align__(16) int id[EO_CHUNK];
-  const int first = blockIdx.y * EO_CHUNK, count = min(EO_CHUNK, n - first), tid = threadIdx.x;
-  if ((int)blockIdx.x * (256 / EO_LANES) >= count) return;
-  for (int j = tid; j < EO_CHUNK; j += 256) id[j] = j < count ? eo_id(ids[first + j], V, padding, status) : 0x7fffffff;
+  if ((int)blockIdx.x >= ctas) return fill(f, blockIdx.x - ctas, gridDim.x - ctas);
+  __shared__ __align__(16) int id[SORT_RANK];
+  const int tid = threadIdx.x;
+  if (blockIdx.x == 0 && tid == 0) *S.join_count = 0;
+  for (int j = tid; j < (n + 3) / 4 * 4; j += SORT_THREADS) id[j] = j < n ? eo_id(ids[j], V, padding, status) : 0x7fffffff;
   __syncthreads();
-  const int i = blockIdx.x * (256 / EO_LANES) + tid / EO_LANES, sub = tid % EO_LANES;
-  const int mine = i < count ? id[i] : 0;
+  const int i = blockIdx.x * (SORT_THREADS / SORT_LANES) + tid / SORT_LANES, sub = tid % SORT_LANES;
+  const int mine = i < n ? id[i] : 0;
   int rank = 0;
-  for (int q = sub; q < (count + 3) / 4; q += EO_LANES) {
+#pragma unroll 4
+  for (int q = sub; q < (n + 3) / 4; q += SORT_LANES) {
     const int4 v = reinterpret_cast<const int4*>(id)[q];
     const int e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int u = 0; u < 4; ++u) rank += e[u] < mine + (4 * q + u < i);
   }
 #pragma unroll
-  for (int o = EO_LANES / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-  if (sub == 0 && i < count) {
-    S.chunk_id[first + rank] = mine;
-    S.chunk_tok[first + rank] = first + i;
+  for (int o = SORT_LANES / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+  if (sub == 0 && i < n) {
+    S.id[rank] = mine;
+    S.tok[rank] = i;
   }
 }
 
+// The first digit's counts of every sort CTA's tokens; the other passes' counts are cleared.
+__global__ void __launch_bounds__(SORT_THREADS)
+embedding_count_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int passes, int bits, int span, int ctas, Fill f, int* status) {
+  rte::after_previous_grid();
+  if ((int)blockIdx.x >= ctas) return fill(f, blockIdx.x - ctas, gridDim.x - ctas);
+  __shared__ int count[1 << SORT_BITS];
+  const int tid = threadIdx.x, bins = 1 << bits;
+  for (int b = tid; b < bins; b += SORT_THREADS) count[b] = 0;
+  if (blockIdx.x == 0 && tid == 0) *S.join_count = 0;
+  __syncthreads();
+  const int begin = blockIdx.x * span, end = min(begin + span, n);
+#pragma unroll 8
+  for (int i = begin + tid; i < end; i += SORT_THREADS) atomicAdd(&count[eo_id(ids[i], V, padding, status) & (bins - 1)], 1);
+  __syncthreads();
+  for (int b = tid; b < bins; b += SORT_THREADS) {
+    S.hist[blockIdx.x * bins + b] = count[b];
+    for (int p = 1; p < passes; ++p) S.hist[(p * ctas + blockIdx.x) * bins + b] = 0;
+  }
+}
+
+// One pass: the tokens of a CTA, SORT_TILE at a time, go to their places by digit `pass`.
+__global__ void __launch_bounds__(SORT_THREADS)
+embedding_place_kernel(const int64_t* __restrict__ ids, const int* __restrict__ id_in, const int* __restrict__ tok_in, int* __restrict__ id_out, int* __restrict__ tok_out,
+                       int* __restrict__ hist, int n, int V, long long padding, int pass, int passes, int bits, int span, int ctas, Fill f) {
+  rte::after_previous_grid();
+  if ((int)blockIdx.x >= ctas) return fill(f, blockIdx.x - ctas, gridDim.x - ctas);
+  constexpr int WARPS = SORT_THREADS / 32, EACH = SORT_TILE / SORT_THREADS, BINS_EACH = (1 << SORT_BITS) / SORT_THREADS;
+  __shared__ int base[1 << SORT_BITS];                             // where the next token of a digit goes
+  __shared__ unsigned short in_warp[WARPS][1 << SORT_BITS];
+  __shared__ int warp_total[WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << bits, shift = pass * bits;
+  {                                                              // a thread has BINS_EACH neighbouring digits
+    const int* h = hist + (size_t)pass * ctas * bins;
+    int total[BINS_EACH] = {}, before[BINS_EACH] = {};
+    const int each = (bins + SORT_THREADS - 1) / SORT_THREADS;
+    for (int u = 0; u < each; ++u) {
+      const int b = tid * each + u;
+      if (b >= bins) break;
+#pragma unroll 16
+      for (int c = 0; c < ctas; ++c) {
+        const int v = h[c * bins + b];
+        total[u] += v;
+        before[u] += c < (int)blockIdx.x ? v : 0;
+      }
+    }
+    int sum = 0;
+#pragma unroll
+    for (int u = 0; u < BINS_EACH; ++u) sum += total[u];
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+    if (lane == 31) warp_total[warp] = upto;
+    __syncthreads();
+    int at = upto - sum;
+    for (int w = 0; w < warp; ++w) at += warp_total[w];
+    for (int u = 0; u < each; ++u) {
+      const int b = tid * each + u;
+      if (b < bins) base[b] = at + before[u];
+      at += total[u];
+    }
+  }
+  const int end = min((int)blockIdx.x * span + span, n);
+  for (int tile = blockIdx.x * span; tile < end; tile += SORT_TILE) {
+    for (int b = tid; b < WARPS * bins; b += SORT_THREADS) in_warp[b >> bits][b & (bins - 1)] = 0;
+    __syncthreads();
+    int id[EACH], tok[EACH], rank[EACH];
+    const int first = tile + warp * 32 * EACH + lane;              // a warp's tokens are neighbours
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = first + 32 * e;
+      id[e] = i < end ? (pass == 0 ? eo_id(ids[i], V, padding, nullptr) : id_in[i]) : -1;
+      tok[e] = i < end ? (pass == 0 ? i : tok_in[i]) : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int digit = id[e] < 0 ? bins : id[e] >> shift & (bins - 1);
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      rank[e] = digit < bins ? in_warp[warp][digit] + __popc(same & ((1u << lane) - 1)) : 0;
+      __syncwarp();
+      if (digit < bins && (same >> lane) == 1) in_warp[warp][digit] += __popc(same);           // (the last of them)
+      __syncwarp();
+    }
+    __syncthreads();
+    int in_tile[BINS_EACH] = {};
+#pragma unroll
+    for (int u = 0; u < BINS_EACH; ++u) {                          // every warp's counts become where its first token goes, within the tile
+      const int b = tid + u * SORT_THREADS;
+      if (b >= bins) break;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) { const int v = in_warp[w][b]; in_warp[w][b] = (unsigned short)in_tile[u]; in_tile[u] += v; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (id[e] < 0) continue;
+      const int digit = id[e] >> shift & (bins - 1), at = base[digit] + in_warp[warp][digit] + rank[e];
+      id_out[at] = id[e];
+      tok_out[at] = tok[e];
+      if (pass + 1 < passes) atomicAdd(&hist[((size_t)(pass + 1) * ctas + at / span) * bins + (id[e] >> (shift + bits) & (bins - 1))], 1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < BINS_EACH; ++u)
+      if (tid + u * SORT_THREADS < bins) base[tid + u * SORT_THREADS] += in_tile[u];
+  }
+}
+
+// ---------------------------------------------------------------- sums
 // how many of the `count` sorted ids are below `limit`
 __device__ __forceinline__ int below(const int* __restrict__ ids, int count, long long limit) {
   int lo = 0, hi = count;
@@ -130,89 +294,121 @@ __device__ __forceinline__ int below(const int* __restrict__ ids, int count, lon
   return lo;
 }
 
-__global__ void __launch_bounds__(256)
-embedding_merge_kernel(EoScratch S, int n) {
-  rte::after_previous_grid();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int chunk = i / EO_CHUNK, id = S.chunk_id[i];
-  int at = i - chunk * EO_CHUNK;
-  for (int c = 0; c * EO_CHUNK < n; ++c)
-    if (c != chunk) at += below(S.chunk_id + c * EO_CHUNK, min(EO_CHUNK, n - c * EO_CHUNK), (long long)id + (c < chunk));
-  S.id[at] = id;
-  S.tok[at] = S.chunk_tok[i];
-}
-
-// blockIdx.x < ranges: a range's sums, its pieces of columns dealt to blockIdx.y; beyond: zeros of 128 table rows that no token names.
+// Groups of tpr threads: one adds the rows of a range, a piece of the columns per thread.  CTAs behind `range_ctas`: zeros of ZERO_ROWS table
+// rows that no token names, where the sort's launches have not filled the table.
+constexpr int ZERO_ROWS = 64, MIN_TPR = 8;
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(128)
-embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pieces, int d, float scale, T* __restrict__ dtable, int ranges) {
+embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pieces, int tpr, int range, int d, float scale, T* __restrict__ dtable, int range_ctas) {
   rte::after_previous_grid();
   using R = typename Raw<T, BYTES>::type;
   using P = Piece<T, BYTES>;
+  __shared__ int ids[128 / MIN_TPR][MAX_RANGE + 2], toks[128 / MIN_TPR][MAX_RANGE];
   R* out = reinterpret_cast<R*>(dtable);
-  const int tid = threadIdx.x;
-  if ((int)blockIdx.x >= ranges) {
-    __shared__ int named[128];
-    const long long v0 = 128LL * (blockIdx.x - ranges);
-    const int v = (int)min(v0 + tid, (long long)V);
-    const int at = below(S.id, n, v);
-    named[tid] = at < n && S.id[at] == v;
+  const int tid = threadIdx.x, groups = 128 / tpr, group = tid / tpr, lane = tid % tpr;
+  if ((int)blockIdx.x >= range_ctas) {
+    int* named = ids[0];                                           // (MAX_RANGE of them)
+    const long long v0 = (long long)ZERO_ROWS * (blockIdx.x - range_ctas);
+    if (tid < ZERO_ROWS) {
+      const int v = (int)min(v0 + tid, (long long)V), at = below(S.id, n, v);
+      named[tid] = at < n && S.id[at] == v;
+    }
     __syncthreads();
-    for (int r = 0; r < 128 && v0 + r < V; ++r)
+    for (int r = group; r < ZERO_ROWS && v0 + r < V; r += groups)
       if (!named[r])
-        for (int c = blockIdx.y * 128 + tid; c < pieces; c += gridDim.y * 128) out[(v0 + r) * pieces + c] = R{};
+        for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) out[(v0 + r) * pieces + c] = R{};
     return;
   }
-  __shared__ int id[EO_RANGE + 2], tok[EO_RANGE];
-  const int a = blockIdx.x * EO_RANGE, count = min(EO_RANGE, n - a);
-  for (int i = tid; i < count + 2; i += 128) {
-    const int at = a - 1 + i;
-    id[i] = at >= 0 && at < n ? S.id[at] : -1;
+  const long long r0 = (long long)blockIdx.x * groups;
+  for (int i = tid; i < groups * (range + 2); i += 128) {
+    const int g = i / (range + 2), e = i % (range + 2);
+    const long long at = (r0 + g) * range - 1 + e;
+    ids[g][e] = at >= 0 && at < n ? S.id[at] : V;                  // (V: takes no gradient)
+    if (e >= 1 && e <= range) toks[g][e - 1] = at < n ? S.tok[at] : 0;
   }
-  for (int i = tid; i < count; i += 128) tok[i] = S.tok[a + i];
   __syncthreads();
+  const int* id = ids[group] + 1;                                  // id[-1], id[range]: the neighbours
+  const int* tok = toks[group];
+  const long long r = r0 + group;
+  int count = 0;                                                   // rows that take a gradient: the first ones
+  while (count < range && id[count] < V) count += count + ROWS_AHEAD <= range && id[count + ROWS_AHEAD - 1] < V ? ROWS_AHEAD : 1;
+  if (count == 0) return;
+  if (lane == 0 && blockIdx.y == 0 && id[range] < V && id[range - 1] == id[range] && !(id[0] == id[range] && id[-1] == id[0]))
+    S.joins[atomicAdd(S.join_count, 1)] = (int)r;
   const R* g = reinterpret_cast<const R*>(dy);
-  for (int c = blockIdx.y * 128 + tid; c < pieces; c += gridDim.y * 128) {
+  for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) {
     P acc;
-    int begin = 0;
-    for (int i = 0; i < count && id[i + 1] < V; ++i) {
-      const P x = unpack<T, BYTES>(g[(long long)tok[i] * pieces + c]);
-      if (i == begin) acc = x;
-      else
+    bool fresh = true, first = true;
+    for (int i0 = 0; i0 < count; i0 += ROWS_AHEAD) {
+      R raw[ROWS_AHEAD];
 #pragma unroll
-        for (int u = 0; u < P::N; ++u) acc.v[u] += x.v[u];
-      if (i + 1 < count && id[i + 2] == id[i + 1]) continue;
-      const bool before = begin == 0 && id[0] == id[1], after = i + 1 == count && id[i + 2] == id[i + 1];
-      if (before || after) {
-        float* p = S.part + ((size_t)blockIdx.x * 2 + !before) * d + c * P::N;
+      for (int u = 0; u < ROWS_AHEAD; ++u)
+        if (i0 + u < count) raw[u] = g[(long long)tok[i0 + u] * pieces + c];
 #pragma unroll
-        for (int u = 0; u < P::N; ++u) p[u] = acc.v[u];
-      } else {
-        out[(long long)id[i + 1] * pieces + c] = pack<T, BYTES>(acc, scale);
+      for (int u = 0; u < ROWS_AHEAD; ++u) {
+        const int i = i0 + u;
+        if (i >= count) break;
+        const P x = unpack<T, BYTES>(raw[u]);
+#pragma unroll
+        for (int w = 0; w < P::N; ++w) acc.v[w] = fresh ? x.v[w] : acc.v[w] + x.v[w];
+        fresh = id[i + 1] != id[i];
+        if (!fresh && i + 1 < range) continue;
+        const bool before = first && id[-1] == id[i];
+        if (before || !fresh) {
+          float* p = S.part + ((size_t)r * 2 + !before) * d + c * P::N;
+#pragma unroll
+          for (int w = 0; w < P::N; ++w) p[w] = acc.v[w];
+        } else {
+          out[(long long)id[i] * pieces + c] = pack<T, BYTES>(acc, scale);
+        }
+        first = false;
       }
-      begin = i + 1;
     }
   }
 }
 
-// The range in which an id begins that reaches beyond it adds what the ranges behind it have of it, in their order.
+// What several ranges have of an id, added in their order: eight warps each take a run of neighbouring ranges, then the warps' sums.
+constexpr int JOIN_WARPS = 8, JOIN_COLUMNS = 128;
 template <typename T>
-__global__ void __launch_bounds__(128)
-embedding_join_kernel(EoScratch S, int n, int V, int d, float scale, T* __restrict__ dtable) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
+embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __restrict__ dtable) {
   rte::after_previous_grid();
-  const int a = blockIdx.x * EO_RANGE, end = a + EO_RANGE;
-  if (end >= n) return;
-  const int v = S.id[end];
-  if (v >= V || S.id[end - 1] != v || (S.id[a] == v && a > 0 && S.id[a - 1] == v)) return;
-  const int last = (below(S.id, n, (long long)v + 1) - 1) / EO_RANGE;
-  for (int c = blockIdx.y * 128 + threadIdx.x; c < d; c += gridDim.y * 128) {
-    float s = S.part[((size_t)blockIdx.x * 2 + 1) * d + c];
-    for (int r = blockIdx.x + 1; r <= last; ++r) s += S.part[(size_t)r * 2 * d + c];
-    dtable[(long long)v * d + c] = (T)(s * scale);
+  __shared__ float sum[JOIN_WARPS][JOIN_COLUMNS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tiles = (d + JOIN_COLUMNS - 1) / JOIN_COLUMNS;
+  const long long jobs = (long long)*S.join_count * tiles;
+  for (long long job = blockIdx.x; job < jobs; job += gridDim.x) {
+    const int r = S.joins[job / tiles], c0 = int(job % tiles) * JOIN_COLUMNS;
+    const long long end = (long long)(r + 1) * range;              // (below n: the id goes on there)
+    const int v = S.id[end];
+    int step = 1;                                                  // the last range that begins with the id: leaps, then halves
+    while (end + (long long)step * range < n && S.id[end + (long long)step * range] == v) step *= 2;
+    int lo = step / 2, hi = step;                                  // range r + 1 + lo begins with it, r + 1 + hi does not
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (end + (long long)mid * range < n && S.id[end + (long long)mid * range] == v) lo = mid; else hi = mid;
+    }
+    const int m = lo + 1, first = int((long long)m * warp / JOIN_WARPS), last = int((long long)m * (warp + 1) / JOIN_WARPS);
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int q = first; q < last; ++q)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + lane + 32 * u < d) a[u] += S.part[(size_t)(r + 1 + q) * 2 * d + c0 + lane + 32 * u];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum[warp][lane + 32 * u] = a[u];
+    __syncthreads();
+    if (tid < JOIN_COLUMNS && c0 + tid < d) {
+      float s = S.part[((size_t)r * 2 + 1) * d + c0 + tid];
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; ++w) s += sum[w][tid];
+      dtable[(long long)v * d + c0 + tid] = (T)(s * scale);
+    }
+    __syncthreads();
   }
 }
 
+// ---------------------------------------------------------------- launches
 bool type_ok(int type) { return type == RTE_TYPE_BF16 || type == RTE_TYPE_F16 || type == RTE_TYPE_F32; }
 // the widest pieces that every row of the two tensors starts on
 int piece_bytes(const void* a, const void* b, long long row_bytes) {
@@ -222,18 +418,45 @@ int piece_bytes(const void* a, const void* b, long long row_bytes) {
 
 template <typename T, int BYTES>
 void launch_fwd(const int64_t* ids, long long n, const void* table, int V, int d, float scale, void* out, int* status, cudaStream_t st) {
-  const int pieces = d * (int)sizeof(T) / BYTES;
-  const long long ctas = rte::ceil_div64(n * pieces, 256);
-  rte::launch(embedding_fwd_kernel<T, BYTES>, (unsigned)(ctas < 148 * 64 ? ctas : 148 * 64), 256, 0, st, ids, n, static_cast<const T*>(table), V, pieces, scale,
+  const int pieces = d * (int)sizeof(T) / BYTES, tpr = threads_per_row(pieces);
+  const long long ctas = rte::ceil_div64(n, (long long)(128 / tpr) * TOKENS_AHEAD);
+  const int columns = (int)min((long long)rte::ceil_div(pieces, tpr), rte::ceil_div64(148 * 8, ctas));      // few tokens: a CTA per 128 pieces
+  rte::launch(embedding_fwd_kernel<T, BYTES>, dim3((unsigned)min(ctas, 148LL * 64), columns), 128, 0, st, ids, n, static_cast<const T*>(table), V, pieces, tpr, scale,
               static_cast<T*>(out), status);
 }
 template <typename T, int BYTES>
-void launch_sum(const void* dy, const EoScratch& s, int n, int V, int d, float scale, void* dtable, cudaStream_t st) {
-  const int pieces = d * (int)sizeof(T) / BYTES, ranges = rte::ceil_div(n, EO_RANGE);
-  const dim3 grid(ranges + rte::ceil_div(V, 128), (unsigned)min(rte::ceil_div(pieces, 128), 64));
-  rte::launch(embedding_sum_kernel<T, BYTES>, grid, 128, 0, st, static_cast<const T*>(dy), s, n, V, pieces, d, scale, static_cast<T*>(dtable), ranges);
-  if (n > EO_RANGE)
-    rte::launch(embedding_join_kernel<T>, dim3(ranges - 1, (unsigned)min(rte::ceil_div(d, 128), 64)), 128, 0, st, s, n, V, d, scale, static_cast<T*>(dtable));
+void launch_sum(const void* dy, const EoScratch& s, int n, int V, int d, float scale, void* dtable, bool filled, cudaStream_t st) {
+  const int pieces = d * (int)sizeof(T) / BYTES, tpr = max(threads_per_row(pieces), MIN_TPR), range = range_of(n), ranges = rte::ceil_div(n, range);
+  const int range_ctas = rte::ceil_div(ranges, 128 / tpr);
+  const dim3 grid(range_ctas + (filled ? 0 : rte::ceil_div(V, ZERO_ROWS)), (unsigned)min(rte::ceil_div(pieces, tpr), 64));
+  rte::launch(embedding_sum_kernel<T, BYTES>, grid, 128, 0, st, static_cast<const T*>(dy), s, n, V, pieces, tpr, range, d, scale, static_cast<T*>(dtable), range_ctas);
+  if (ranges > 1)
+    rte::launch(embedding_join_kernel<T>, min(rte::ceil_div64((long long)(ranges - 1) * d, JOIN_COLUMNS), 148LL * 4), 32 * JOIN_WARPS, 0, st, s, n, range, d, scale,
+                static_cast<T*>(dtable));
+}
+
+// id and tok sorted; `table` (NULL: not) filled with zeros on the way.
+void launch_sort(const int64_t* ids, int n, int V, long long padding, const EoScratch& s, char* table, long long table_bytes, int* status, cudaStream_t st) {
+  const Digits dg = n > SORT_RANK ? digits_of(V) : Digits{0, 0};
+  const int launches = 1 + dg.passes, fills = table ? 2 * 148 : 0;
+  const long long part = table ? rte::ceil_div64(rte::ceil_div64(table_bytes, launches), 256) * 256 : 0;
+  auto slice = [&](int i) { const long long at = min(i * part, table_bytes); return Fill{table + at, min(part, table_bytes - at)}; };
+  if (dg.passes == 0) {
+    const int ctas = rte::ceil_div(n, SORT_THREADS / SORT_LANES);
+    rte::launch(embedding_rank_kernel, ctas + fills, SORT_THREADS, 0, st, ids, n, V, padding, s, slice(0), ctas, status);
+    return;
+  }
+  const int span = sort_span(n), ctas = rte::ceil_div(n, span);
+  rte::launch(embedding_count_kernel, ctas + fills, SORT_THREADS, 0, st, ids, n, V, padding, s, dg.passes, dg.bits, span, ctas, slice(0), status);
+  const int *id = nullptr, *tok = nullptr;
+  for (int p = 0; p < dg.passes; ++p) {
+    const bool to_first = (dg.passes - 1 - p) % 2 == 0;
+    int *id_out = to_first ? s.id : s.id2, *tok_out = to_first ? s.tok : s.tok2;
+    rte::launch(embedding_place_kernel, ctas + fills, SORT_THREADS, 0, st, ids, id, tok, id_out, tok_out, s.hist, n, V, padding, p, dg.passes, dg.bits, span, ctas,
+                slice(1 + p));
+    id = id_out;
+    tok = tok_out;
+  }
 }
 
 }  // namespace
@@ -284,10 +507,10 @@ extern "C" int rte_embedding_bwd(const int64_t* ids, int64_t n, const void* dy, 
   if (type == RTE_TYPE_F32 && bytes < 4) return RTE_ERR_ALIGNMENT;
   EoScratch s;
   eo_layout(static_cast<char*>(scratch), n, d, &s);
-  const int chunks = (int)rte::ceil_div64(n, EO_CHUNK), in_chunk = (int)(n < EO_CHUNK ? n : EO_CHUNK);
-  rte::launch(embedding_rank_kernel, dim3(rte::ceil_div(in_chunk, 256 / EO_LANES), chunks), 256, 0, ST(stream), ids, (int)n, V, padding_idx, s, status);
-  if (chunks > 1) rte::launch(embedding_merge_kernel, (unsigned)rte::ceil_div64(n, 256), 256, 0, ST(stream), s, (int)n);
-#define CALL(T, B) launch_sum<T, B>(dy, s, (int)n, V, d, scale, dtable, ST(stream))
+  // Rows that no token names: with fewer tokens than rows the whole table is filled beside the sort, and the named rows are written again.
+  const bool fill_ahead = n <= V;
+  launch_sort(ids, (int)n, V, padding_idx, s, fill_ahead ? static_cast<char*>(dtable) : nullptr, (long long)V * d * (type == RTE_TYPE_F32 ? 4 : 2), status, ST(stream));
+#define CALL(T, B) launch_sum<T, B>(dy, s, (int)n, V, d, scale, dtable, fill_ahead, ST(stream))
   BY_PIECE(type, bytes, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
