@@ -4,12 +4,13 @@
 //
 // The gradient's addends meet in the order of the tokens, whatever the launch: the token positions are sorted by (id, position), a
 // thread adds its columns of a range of consecutive sorted rows, what a range adds for an id that reaches beyond it goes to a
-// partial, and those of one id are added in order.  No atomics on values; rows that no token names are zeros.
+// partial, and those of one id are added in order; an id that ends within the next range is finished by the one in which it
+// begins.  No atomics on values; rows that no token names are zeros.
 //
-// The sort: up to SORT_RANK tokens each counts the tokens that come before it.  More take a pass per digit of the id (two digits of up to 10
-// bits for tables of up to 2^20 rows), each stable: a CTA's tokens are counted by digit, and a token's place is the number of
-// tokens with a smaller digit, those with its own in CTAs before, in warps before, and in its warp before it.  A pass leaves the next digit's
-// counts behind, so that a sort of two digits is three launches.
+// The sort takes a pass per digit of the id, each stable: a token's place is the number of tokens with a smaller digit, those with its own
+// in CTAs before, in warps before, and in its warp before it.  Up to SORT_ONE tokens are sorted in one CTA's shared memory (digits of up to
+// 8 bits).  More are counted by CTAs, and a pass leaves the next digit's counts behind, so that a sort of two digits (of up to 10 bits: tables
+// of up to 2^20 rows) is three launches.
 
 #include <cuda_fp16.h>
 
@@ -17,8 +18,8 @@
 
 namespace {
 
-constexpr int SORT_RANK = 2048, SORT_LANES = 8;                      // tokens that are ranked by counting, threads that count for one
-constexpr int SORT_THREADS = 256, SORT_TILE = 2048, SORT_CTAS = 296; // tokens a CTA places at a time; CTAs at most
+constexpr int SORT_ONE = 8192, ONE_THREADS = 1024, ONE_BITS = 8;      // tokens that one CTA sorts, its threads, the bits of its digits
+constexpr int SORT_THREADS = 256, SORT_CTAS = 296;                   // of a sort's launch; CTAs at most
 constexpr int SORT_BITS = 10;                                        // of a digit, at most
 constexpr int ROWS_AHEAD = 8, MAX_RANGE = 64;                        // rows a thread has in flight; sorted rows of a range at most
 
@@ -93,27 +94,33 @@ embedding_fwd_kernel(const int64_t* __restrict__ ids, long long n, const T* __re
 
 // ---------------------------------------------------------------- the gradient's workspace
 struct Digits { int passes, bits; };           // of ids 0 .. V (V: takes no gradient)
-Digits digits_of(int V) {
+Digits digits_of(int V, int most) {
   int b = 1;
   while (b < 31 && V >> b) ++b;
-  const int passes = b <= SORT_BITS ? 1 : (b + SORT_BITS - 1) / SORT_BITS;
+  const int passes = (b + most - 1) / most;
   return {passes, (b + passes - 1) / passes};
 }
 struct EoScratch {
   int *id, *tok;                // [n]: sorted
   int *id2, *tok2;              // [n]: between passes
   int* hist;                    // [passes][sort CTAs][1 << bits]
-  int *joins, *join_count;      // ranges whose last id goes on behind them and did not begin before them
+  int2* joins;                  // (range, id): ranges in which an id begins that fills the next one too and goes on
+  int* join_count;
   float* part;                  // [ranges][2][d]: what a range adds for an id that began before it | that goes on behind it
 };
-int sort_span(long long n) { return (int)rte::ceil_div64(rte::ceil_div64(n, SORT_TILE), SORT_CTAS) * SORT_TILE; }      // tokens of a sort CTA
-int range_of(long long n) { return n >= 32768 ? MAX_RANGE : 32; }
+// Tokens that a thread of a sort CTA places at a time: few while the CTAs are few (all of them read all of their counts).
+int sort_each(long long n) { return n <= 32768 ? 2 : n <= 65536 ? 4 : 8; }
+int sort_span(long long n) {                                          // tokens of a sort CTA
+  const int tile = SORT_THREADS * sort_each(n);
+  return (int)rte::ceil_div64(rte::ceil_div64(n, tile), SORT_CTAS) * tile;
+}
+int range_of(long long n) { return n >= 65536 ? MAX_RANGE : n >= 32768 ? 32 : n >= 16384 ? 16 : 8; }
 size_t eo_layout(char* at, long long n, int d, EoScratch* s) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t list = up((size_t)n * 4), ranges = (size_t)rte::ceil_div64(n, range_of(n));
   // (three digits of 10 bits and one more pass: what a table of any size takes)
-  const size_t hist = n > SORT_RANK ? up((size_t)4 * rte::ceil_div64(n, sort_span(n)) * (1 << SORT_BITS) * 4) : 0;
-  const size_t lists = n > SORT_RANK ? 4 : 2;
+  const size_t hist = n > SORT_ONE ? up((size_t)4 * rte::ceil_div64(n, sort_span(n)) * (1 << SORT_BITS) * 4) : 0;
+  const size_t lists = n > SORT_ONE ? 4 : 2;
   if (s) {
     s->id = reinterpret_cast<int*>(at);
     s->tok = reinterpret_cast<int*>(at + list);
@@ -121,10 +128,10 @@ size_t eo_layout(char* at, long long n, int d, EoScratch* s) {
     s->tok2 = reinterpret_cast<int*>(at + 3 * list);
     s->hist = reinterpret_cast<int*>(at + lists * list);
     s->join_count = reinterpret_cast<int*>(at + lists * list + hist);
-    s->joins = s->join_count + 64;
-    s->part = reinterpret_cast<float*>(at + lists * list + hist + 256 + up(ranges * 4));
+    s->joins = reinterpret_cast<int2*>(s->join_count + 64);
+    s->part = reinterpret_cast<float*>(at + lists * list + hist + 256 + up(ranges * 8));
   }
-  return lists * list + hist + 256 + up(ranges * 4) + up(ranges * 2 * d * 4);
+  return lists * list + hist + 256 + up(ranges * 8) + up(ranges * 2 * d * 4);
 }
 
 // Ids that take no gradient (padding, out of range) count as V: behind all others.
@@ -148,31 +155,84 @@ __device__ __forceinline__ void fill(const Fill& f, int cta, int ctas) {
 }
 
 // ---------------------------------------------------------------- sort
-// Up to SORT_RANK tokens: a CTA places SORT_THREADS / SORT_LANES of them.
-__global__ void __launch_bounds__(SORT_THREADS)
-embedding_rank_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, Fill f, int ctas, int* status) {
+// Up to SORT_ONE tokens, all passes in shared memory: id | tok of a pass and of the next, the warps' counts.
+__host__ __device__ constexpr size_t one_bytes(int n) { return (size_t)4 * ((n + 3) / 4 * 4) * 4 + (size_t)(ONE_THREADS / 32) * (1 << ONE_BITS) * 2; }
+__global__ void __launch_bounds__(ONE_THREADS)
+embedding_sort_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int passes, int bits, Fill f, int* status) {
   rte::after_previous_grid();
-  if ((int)blockIdx.x >= ctas) return fill(f, blockIdx.x - ctas, gridDim.x - ctas);
-  __shared__ __align__(16) int id[SORT_RANK];
-  const int tid = threadIdx.x;
-  if (blockIdx.x == 0 && tid == 0) *S.join_count = 0;
-  for (int j = tid; j < (n + 3) / 4 * 4; j += SORT_THREADS) id[j] = j < n ? eo_id(ids[j], V, padding, status) : 0x7fffffff;
-  __syncthreads();
-  const int i = blockIdx.x * (SORT_THREADS / SORT_LANES) + tid / SORT_LANES, sub = tid % SORT_LANES;
-  const int mine = i < n ? id[i] : 0;
-  int rank = 0;
-#pragma unroll 4
-  for (int q = sub; q < (n + 3) / 4; q += SORT_LANES) {
-    const int4 v = reinterpret_cast<const int4*>(id)[q];
-    const int e[4] = {v.x, v.y, v.z, v.w};
+  if (blockIdx.x >= 1) return fill(f, blockIdx.x - 1, gridDim.x - 1);
+  constexpr int WARPS = ONE_THREADS / 32, EACH = SORT_ONE / ONE_THREADS, BINS = 1 << ONE_BITS, SHARE = ONE_THREADS / BINS;
+  extern __shared__ __align__(16) int one_shared[];
+  __shared__ int base[BINS], warp_total[BINS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pad = (n + 3) / 4 * 4;
+  int *id_at[2] = {one_shared, one_shared + 2 * pad}, *tok_at[2] = {one_shared + pad, one_shared + 3 * pad};
+  unsigned short(*in_warp)[BINS] = reinterpret_cast<unsigned short(*)[BINS]>(one_shared + 4 * pad);
+  if (tid == 0) *S.join_count = 0;
+  for (int i = tid; i < n; i += ONE_THREADS) { id_at[0][i] = eo_id(ids[i], V, padding, status); tok_at[0][i] = i; }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits, from = pass & 1;
+    for (int i = tid; i < WARPS * BINS / 8; i += ONE_THREADS) reinterpret_cast<uint4*>(in_warp)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    int id[EACH], tok[EACH], rank[EACH];
+    const int first = warp * 32 * EACH + lane;                     // a warp's tokens are neighbours
 #pragma unroll
-    for (int u = 0; u < 4; ++u) rank += e[u] < mine + (4 * q + u < i);
-  }
+    for (int e = 0; e < EACH; ++e) id[e] = -1;
 #pragma unroll
-  for (int o = SORT_LANES / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-  if (sub == 0 && i < n) {
-    S.id[rank] = mine;
-    S.tok[rank] = i;
+    for (int e = 0; e < EACH; ++e) {
+      const int i = first + 32 * e;
+      if (i - lane >= n) break;
+      id[e] = i < n ? id_at[from][i] : -1;
+      tok[e] = i < n ? tok_at[from][i] : 0;
+      const int digit = id[e] < 0 ? BINS : id[e] >> shift & ((1 << bits) - 1);
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      rank[e] = digit < BINS ? in_warp[warp][digit] + __popc(same & ((1u << lane) - 1)) : 0;
+      __syncwarp();
+      if (digit < BINS && same >> lane == 1) in_warp[warp][digit] += __popc(same);             // (the last of them)
+      __syncwarp();
+    }
+    __syncthreads();
+    {                                                              // SHARE threads a digit, each WARPS / SHARE warps' counts
+      const int digit = tid / SHARE, part = tid % SHARE;
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS / SHARE; ++w) sum += in_warp[part * (WARPS / SHARE) + w][digit];
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < SHARE; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (part >= o) upto += v; }
+      int at = upto - sum;
+#pragma unroll
+      for (int w = 0; w < WARPS / SHARE; ++w) {
+        unsigned short& c = in_warp[part * (WARPS / SHARE) + w][digit];
+        const int v = c;
+        c = (unsigned short)at;
+        at += v;
+      }
+      if (part == SHARE - 1) base[digit] = upto;
+    }
+    __syncthreads();
+    int v = 0, total = 0;
+    if (tid < BINS) {
+      total = v = base[tid];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += u; }
+      if (lane == 31) warp_total[warp] = v;
+    }
+    __syncthreads();
+    if (tid < BINS) {
+      int at = v - total;
+      for (int w = 0; w < warp; ++w) at += warp_total[w];
+      base[tid] = at;
+    }
+    __syncthreads();
+    int *id_out = pass + 1 < passes ? id_at[from ^ 1] : S.id, *tok_out = pass + 1 < passes ? tok_at[from ^ 1] : S.tok;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (id[e] < 0) continue;
+      const int digit = id[e] >> shift & ((1 << bits) - 1), at = base[digit] + in_warp[warp][digit] + rank[e];
+      id_out[at] = id[e];
+      tok_out[at] = tok[e];
+    }
+    __syncthreads();
   }
 }
 
@@ -196,13 +256,14 @@ embedding_count_kernel(const int64_t* __restrict__ ids, int n, int V, long long 
   }
 }
 
-// One pass: the tokens of a CTA, SORT_TILE at a time, go to their places by digit `pass`.
+// One pass: the tokens of a CTA, EACH per thread at a time, go to their places by digit `pass`.
+template <int EACH>
 __global__ void __launch_bounds__(SORT_THREADS)
 embedding_place_kernel(const int64_t* __restrict__ ids, const int* __restrict__ id_in, const int* __restrict__ tok_in, int* __restrict__ id_out, int* __restrict__ tok_out,
                        int* __restrict__ hist, int n, int V, long long padding, int pass, int passes, int bits, int span, int ctas, Fill f) {
   rte::after_previous_grid();
   if ((int)blockIdx.x >= ctas) return fill(f, blockIdx.x - ctas, gridDim.x - ctas);
-  constexpr int WARPS = SORT_THREADS / 32, EACH = SORT_TILE / SORT_THREADS, BINS_EACH = (1 << SORT_BITS) / SORT_THREADS;
+  constexpr int WARPS = SORT_THREADS / 32, TILE = SORT_THREADS * EACH, BINS_EACH = (1 << SORT_BITS) / SORT_THREADS;
   __shared__ int base[1 << SORT_BITS];                             // where the next token of a digit goes
   __shared__ unsigned short in_warp[WARPS][1 << SORT_BITS];
   __shared__ int warp_total[WARPS];
@@ -238,7 +299,7 @@ embedding_place_kernel(const int64_t* __restrict__ ids, const int* __restrict__ 
     }
   }
   const int end = min((int)blockIdx.x * span + span, n);
-  for (int tile = blockIdx.x * span; tile < end; tile += SORT_TILE) {
+  for (int tile = blockIdx.x * span; tile < end; tile += TILE) {
     for (int b = tid; b < WARPS * bins; b += SORT_THREADS) in_warp[b >> bits][b & (bins - 1)] = 0;
     __syncthreads();
     int id[EACH], tok[EACH], rank[EACH];
@@ -303,7 +364,7 @@ embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pi
   rte::after_previous_grid();
   using R = typename Raw<T, BYTES>::type;
   using P = Piece<T, BYTES>;
-  __shared__ int ids[128 / MIN_TPR][MAX_RANGE + 2], toks[128 / MIN_TPR][MAX_RANGE];
+  __shared__ int ids[128 / MIN_TPR][2 * MAX_RANGE + 2], toks[128 / MIN_TPR][2 * MAX_RANGE];
   R* out = reinterpret_cast<R*>(dtable);
   const int tid = threadIdx.x, groups = 128 / tpr, group = tid / tpr, lane = tid % tpr;
   if ((int)blockIdx.x >= range_ctas) {
@@ -320,39 +381,47 @@ embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pi
     return;
   }
   const long long r0 = (long long)blockIdx.x * groups;
-  for (int i = tid; i < groups * (range + 2); i += 128) {
-    const int g = i / (range + 2), e = i % (range + 2);
+  for (int i = tid; i < groups * (2 * range + 2); i += 128) {
+    const int g = i / (2 * range + 2), e = i % (2 * range + 2);
     const long long at = (r0 + g) * range - 1 + e;
     ids[g][e] = at >= 0 && at < n ? S.id[at] : V;                  // (V: takes no gradient)
-    if (e >= 1 && e <= range) toks[g][e - 1] = at < n ? S.tok[at] : 0;
+    if (e >= 1 && e <= 2 * range) toks[g][e - 1] = at < n ? S.tok[at] : 0;
   }
-  __syncthreads();
-  const int* id = ids[group] + 1;                                  // id[-1], id[range]: the neighbours
-  const int* tok = toks[group];
   const long long r = r0 + group;
-  int count = 0;                                                   // rows that take a gradient: the first ones
-  while (count < range && id[count] < V) count += count + ROWS_AHEAD <= range && id[count + ROWS_AHEAD - 1] < V ? ROWS_AHEAD : 1;
-  if (count == 0) return;
-  if (lane == 0 && blockIdx.y == 0 && id[range] < V && id[range - 1] == id[range] && !(id[0] == id[range] && id[-1] == id[0]))
-    S.joins[atomicAdd(S.join_count, 1)] = (int)r;
+  const int before_last = r >= 1 && (r - 1) * range - 1 >= 0 && (r - 1) * range - 1 < n ? S.id[(r - 1) * range - 1] : V;
+  __syncthreads();
+  const int* id = ids[group] + 1;                                  // id[-1], id[range ..]: the neighbours
+  const int* tok = toks[group];
+  int begin = 0, end = 0;                                          // rows that are added here; those that take a gradient come first
+  while (end < range && id[end] < V) end += end + ROWS_AHEAD <= range && id[end + ROWS_AHEAD - 1] < V ? ROWS_AHEAD : 1;
+  if (id[-1] == id[0] && id[range] != id[0] && before_last != id[0])        // the range before finishes what it began
+    while (begin < end && id[begin] == id[-1]) ++begin;
+  const int last = id[range - 1];
+  if (last < V && last == id[range] && !(id[0] == last && id[-1] == last)) {      // begins here and goes on:
+    if (id[2 * range] != last) {                                   // to be finished here,
+      while (id[end] == last) ++end;
+    } else if (lane == 0 && blockIdx.y == 0) {                     // or over a whole range and further, to be joined
+      S.joins[atomicAdd(S.join_count, 1)] = make_int2((int)r, last);
+    }
+  }
   const R* g = reinterpret_cast<const R*>(dy);
   for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) {
     P acc;
-    bool fresh = true, first = true;
-    for (int i0 = 0; i0 < count; i0 += ROWS_AHEAD) {
+    bool fresh = true, first = begin == 0;
+    for (int i0 = begin; i0 < end; i0 += ROWS_AHEAD) {
       R raw[ROWS_AHEAD];
 #pragma unroll
       for (int u = 0; u < ROWS_AHEAD; ++u)
-        if (i0 + u < count) raw[u] = g[(long long)tok[i0 + u] * pieces + c];
+        if (i0 + u < end) raw[u] = g[(long long)tok[i0 + u] * pieces + c];
 #pragma unroll
       for (int u = 0; u < ROWS_AHEAD; ++u) {
         const int i = i0 + u;
-        if (i >= count) break;
+        if (i >= end) break;
         const P x = unpack<T, BYTES>(raw[u]);
 #pragma unroll
         for (int w = 0; w < P::N; ++w) acc.v[w] = fresh ? x.v[w] : acc.v[w] + x.v[w];
         fresh = id[i + 1] != id[i];
-        if (!fresh && i + 1 < range) continue;
+        if (!fresh && i + 1 < end) continue;
         const bool before = first && id[-1] == id[i];
         if (before || !fresh) {
           float* p = S.part + ((size_t)r * 2 + !before) * d + c * P::N;
@@ -378,17 +447,24 @@ embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __re
   const int tiles = (d + JOIN_COLUMNS - 1) / JOIN_COLUMNS;
   const long long jobs = (long long)*S.join_count * tiles;
   for (long long job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const int r = S.joins[job / tiles], c0 = int(job % tiles) * JOIN_COLUMNS;
-    const long long end = (long long)(r + 1) * range;              // (below n: the id goes on there)
-    const int v = S.id[end];
-    int step = 1;                                                  // the last range that begins with the id: leaps, then halves
-    while (end + (long long)step * range < n && S.id[end + (long long)step * range] == v) step *= 2;
-    int lo = step / 2, hi = step;                                  // range r + 1 + lo begins with it, r + 1 + hi does not
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (end + (long long)mid * range < n && S.id[end + (long long)mid * range] == v) lo = mid; else hi = mid;
+    const int2 join = S.joins[job / tiles];
+    const int r = join.x, v = join.y, c0 = int(job % tiles) * JOIN_COLUMNS;
+    // how many ranges behind r + 1 begin with the id: leaps of 1024, 32 and one range, a lane each, asked for at once
+    const auto begins = [&](long long q) { const long long at = (r + 1 + q) * (long long)range; return at < n && S.id[at] == v; };
+    int m = 0;
+    bool near = begins(lane + 1), mid = begins(32LL * (lane + 1)), far = begins(1024LL * (lane + 1));
+    int c = __popc(__ballot_sync(0xffffffffu, far));
+    while (c == 32) {
+      m += 32 * 1024;
+      c = __popc(__ballot_sync(0xffffffffu, begins(m + 1024LL * (lane + 1))));
     }
-    const int m = lo + 1, first = int((long long)m * warp / JOIN_WARPS), last = int((long long)m * (warp + 1) / JOIN_WARPS);
+    m += c * 1024;
+    if (m > 0) mid = begins(m + 32LL * (lane + 1));
+    c = __popc(__ballot_sync(0xffffffffu, mid));                   // (fewer than 32: range m + 1024 does not)
+    m += c * 32;
+    if (m > 0) near = begins(m + lane + 1);
+    m += __popc(__ballot_sync(0xffffffffu, near)) + 1;             // r + 1 .. r + m
+    const int first = int((long long)m * warp / JOIN_WARPS), last = int((long long)m * (warp + 1) / JOIN_WARPS);
     float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int q = first; q < last; ++q)
@@ -431,19 +507,19 @@ void launch_sum(const void* dy, const EoScratch& s, int n, int V, int d, float s
   const dim3 grid(range_ctas + (filled ? 0 : rte::ceil_div(V, ZERO_ROWS)), (unsigned)min(rte::ceil_div(pieces, tpr), 64));
   rte::launch(embedding_sum_kernel<T, BYTES>, grid, 128, 0, st, static_cast<const T*>(dy), s, n, V, pieces, tpr, range, d, scale, static_cast<T*>(dtable), range_ctas);
   if (ranges > 1)
-    rte::launch(embedding_join_kernel<T>, min(rte::ceil_div64((long long)(ranges - 1) * d, JOIN_COLUMNS), 148LL * 4), 32 * JOIN_WARPS, 0, st, s, n, range, d, scale,
+    rte::launch(embedding_join_kernel<T>, min(rte::ceil_div64((long long)(ranges - 1) * d, JOIN_COLUMNS), 148LL * 8), 32 * JOIN_WARPS, 0, st, s, n, range, d, scale,
                 static_cast<T*>(dtable));
 }
 
 // id and tok sorted; `table` (NULL: not) filled with zeros on the way.
 void launch_sort(const int64_t* ids, int n, int V, long long padding, const EoScratch& s, char* table, long long table_bytes, int* status, cudaStream_t st) {
-  const Digits dg = n > SORT_RANK ? digits_of(V) : Digits{0, 0};
-  const int launches = 1 + dg.passes, fills = table ? 2 * 148 : 0;
+  const bool one = n <= SORT_ONE;
+  const Digits dg = digits_of(V, one ? ONE_BITS : SORT_BITS);
+  const int launches = one ? 1 : 1 + dg.passes, fills = table ? (one ? 147 : 2 * 148) : 0;
   const long long part = table ? rte::ceil_div64(rte::ceil_div64(table_bytes, launches), 256) * 256 : 0;
   auto slice = [&](int i) { const long long at = min(i * part, table_bytes); return Fill{table + at, min(part, table_bytes - at)}; };
-  if (dg.passes == 0) {
-    const int ctas = rte::ceil_div(n, SORT_THREADS / SORT_LANES);
-    rte::launch(embedding_rank_kernel, ctas + fills, SORT_THREADS, 0, st, ids, n, V, padding, s, slice(0), ctas, status);
+  if (one) {
+    rte::launch(embedding_sort_kernel, 1 + fills, ONE_THREADS, one_bytes(n), st, ids, n, V, padding, s, dg.passes, dg.bits, slice(0), status);
     return;
   }
   const int span = sort_span(n), ctas = rte::ceil_div(n, span);
@@ -452,7 +528,8 @@ void launch_sort(const int64_t* ids, int n, int V, long long padding, const EoSc
   for (int p = 0; p < dg.passes; ++p) {
     const bool to_first = (dg.passes - 1 - p) % 2 == 0;
     int *id_out = to_first ? s.id : s.id2, *tok_out = to_first ? s.tok : s.tok2;
-    rte::launch(embedding_place_kernel, ctas + fills, SORT_THREADS, 0, st, ids, id, tok, id_out, tok_out, s.hist, n, V, padding, p, dg.passes, dg.bits, span, ctas,
+    const auto place = sort_each(n) == 2 ? embedding_place_kernel<2> : sort_each(n) == 4 ? embedding_place_kernel<4> : embedding_place_kernel<8>;
+    rte::launch(place, ctas + fills, SORT_THREADS, 0, st, ids, id, tok, id_out, tok_out, s.hist, n, V, padding, p, dg.passes, dg.bits, span, ctas,
                 slice(1 + p));
     id = id_out;
     tok = tok_out;
@@ -507,6 +584,8 @@ extern "C" int rte_embedding_bwd(const int64_t* ids, int64_t n, const void* dy, 
   if (type == RTE_TYPE_F32 && bytes < 4) return RTE_ERR_ALIGNMENT;
   EoScratch s;
   eo_layout(static_cast<char*>(scratch), n, d, &s);
+  if (n <= SORT_ONE && cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one_bytes(SORT_ONE)) != cudaSuccess)
+    return RTE_ERR_LAUNCH;
   // Rows that no token names: with fewer tokens than rows the whole table is filled beside the sort, and the named rows are written again.
   const bool fill_ahead = n <= V;
   launch_sort(ids, (int)n, V, padding_idx, s, fill_ahead ? static_cast<char*>(dtable) : nullptr, (long long)V * d * (type == RTE_TYPE_F32 ? 4 : 2), status, ST(stream));
