@@ -8,17 +8,20 @@
 // begins.  No atomics on values; rows that no token names are zeros.
 //
 // The sort takes a pass per digit of the id, each stable: a token's place is the number of tokens with a smaller digit, those with its own
-// in CTAs before, in warps before, and in its warp before it.  Up to SORT_ONE tokens are sorted in one CTA's shared memory (digits of up to
-// 8 bits).  More are counted by CTAs, and a pass leaves the next digit's counts behind, so that a sort of two digits (of up to 10 bits: tables
+// in CTAs before, in warps before, and in its warp before it.  Up to SORT_ONE tokens are one cluster's, which exchanges its CTAs' counts
+// (digits of up to 8 bits, all passes in one launch).  More are counted by CTAs, and a pass leaves the next digit's counts behind, so that a sort of two digits (of up to 10 bits: tables
 // of up to 2^20 rows) is three launches.
 
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "rte_common.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace {
 
-constexpr int SORT_ONE = 8192, ONE_THREADS = 1024, ONE_BITS = 8;      // tokens that one CTA sorts, its threads, the bits of its digits
+constexpr int SORT_ONE = 8192, ONE_CTAS = 8, ONE_BITS = 8;           // tokens that one cluster sorts, its CTAs, the bits of its digits
 constexpr int SORT_THREADS = 256, SORT_CTAS = 296;                   // of a sort's launch; CTAs at most
 constexpr int SORT_BITS = 10;                                        // of a digit, at most
 constexpr int ROWS_AHEAD = 8, MAX_RANGE = 64;                        // rows a thread has in flight; sorted rows of a range at most
@@ -114,13 +117,13 @@ int sort_span(long long n) {                                          // tokens 
   const int tile = SORT_THREADS * sort_each(n);
   return (int)rte::ceil_div64(rte::ceil_div64(n, tile), SORT_CTAS) * tile;
 }
-int range_of(long long n) { return n >= 65536 ? MAX_RANGE : n >= 32768 ? 32 : n >= 16384 ? 16 : 8; }
+int range_of(long long n) { return n >= 65536 ? MAX_RANGE : n >= 32768 ? 32 : n >= 8192 ? 16 : 8; }
 size_t eo_layout(char* at, long long n, int d, EoScratch* s) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t list = up((size_t)n * 4), ranges = (size_t)rte::ceil_div64(n, range_of(n));
   // (three digits of 10 bits and one more pass: what a table of any size takes)
   const size_t hist = n > SORT_ONE ? up((size_t)4 * rte::ceil_div64(n, sort_span(n)) * (1 << SORT_BITS) * 4) : 0;
-  const size_t lists = n > SORT_ONE ? 4 : 2;
+  const size_t lists = 4;
   if (s) {
     s->id = reinterpret_cast<int*>(at);
     s->tok = reinterpret_cast<int*>(at + list);
@@ -155,76 +158,99 @@ __device__ __forceinline__ void fill(const Fill& f, int cta, int ctas) {
 }
 
 // ---------------------------------------------------------------- sort
-// Up to SORT_ONE tokens, all passes in shared memory: id | tok of a pass and of the next, the warps' counts.
-__host__ __device__ constexpr size_t one_bytes(int n) { return (size_t)4 * ((n + 3) / 4 * 4) * 4 + (size_t)(ONE_THREADS / 32) * (1 << ONE_BITS) * 2; }
-__global__ void __launch_bounds__(ONE_THREADS)
+// The lanes with this lane's digit (of `bits` bits), those that bring none apart: a vote per bit.
+__device__ __forceinline__ uint32_t same_digit(int digit, bool brings, int bits) {
+  uint32_t same = __ballot_sync(0xffffffffu, brings);
+  if (!brings) same = ~same;
+#pragma unroll
+  for (int b = 0; b < SORT_BITS; ++b) {
+    if (b >= bits) break;
+    const bool one = digit >> b & 1;
+    const uint32_t ones = __ballot_sync(0xffffffffu, one);
+    same &= one ? ones : ~ones;
+  }
+  return same;
+}
+// Exclusive sums over the block's threads.
+__device__ __forceinline__ int sums_before(int v, int* warp_total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += u; }
+  if (lane == 31) warp_total[warp] = upto;
+  __syncthreads();
+  int at = upto - v;
+  for (int w = 0; w < warp; ++w) at += warp_total[w];
+  return at;
+}
+
+// Up to SORT_ONE tokens by the first cluster, a run of neighbouring tokens per CTA; the other clusters fill.  One CTA of 1024 threads took
+// 21 us for 8192 tokens, most of it the rounds of votes on one SM.
+__global__ void __cluster_dims__(ONE_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
 embedding_sort_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int passes, int bits, Fill f, int* status) {
   rte::after_previous_grid();
-  if (blockIdx.x >= 1) return fill(f, blockIdx.x - 1, gridDim.x - 1);
-  constexpr int WARPS = ONE_THREADS / 32, EACH = SORT_ONE / ONE_THREADS, BINS = 1 << ONE_BITS, SHARE = ONE_THREADS / BINS;
-  extern __shared__ __align__(16) int one_shared[];
-  __shared__ int base[BINS], warp_total[BINS / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pad = (n + 3) / 4 * 4;
-  int *id_at[2] = {one_shared, one_shared + 2 * pad}, *tok_at[2] = {one_shared + pad, one_shared + 3 * pad};
-  unsigned short(*in_warp)[BINS] = reinterpret_cast<unsigned short(*)[BINS]>(one_shared + 4 * pad);
-  if (tid == 0) *S.join_count = 0;
-  for (int i = tid; i < n; i += ONE_THREADS) { id_at[0][i] = eo_id(ids[i], V, padding, status); tok_at[0][i] = i; }
+  if (blockIdx.x >= ONE_CTAS) return fill(f, blockIdx.x - ONE_CTAS, gridDim.x - ONE_CTAS);
+  constexpr int WARPS = SORT_THREADS / 32, EACH = SORT_ONE / ONE_CTAS / SORT_THREADS, BINS = 1 << ONE_BITS;
+  static_assert(BINS == SORT_THREADS, "a thread per digit");
+  __shared__ int base[BINS], count[BINS], warp_total[WARPS];
+  __shared__ unsigned short in_warp[WARPS][BINS];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank_in = (int)cluster.block_rank();
+  const int each = (n + ONE_CTAS * SORT_THREADS - 1) / (ONE_CTAS * SORT_THREADS);      // rounds of a warp
+  const int first = (rank_in * WARPS + warp) * 32 * each + lane;     // a warp's tokens are neighbours
+  if (blockIdx.x == 0 && tid == 0) *S.join_count = 0;
+  int id[EACH], tok[EACH], rank[EACH];
   for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * bits, from = pass & 1;
-    for (int i = tid; i < WARPS * BINS / 8; i += ONE_THREADS) reinterpret_cast<uint4*>(in_warp)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    int id[EACH], tok[EACH], rank[EACH];
-    const int first = warp * 32 * EACH + lane;                     // a warp's tokens are neighbours
+    const int shift = pass * bits;
+    const bool to_first = (passes - 1 - pass) % 2 == 0;
+    int *id_out = to_first ? S.id : S.id2, *tok_out = to_first ? S.tok : S.tok2;
+    const int *id_in = to_first ? S.id2 : S.id, *tok_in = to_first ? S.tok2 : S.tok;
+    if (pass == 0) {
+      int64_t v[EACH];                                               // (all requested before the first is looked at)
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) id[e] = -1;
+      for (int e = 0; e < EACH; ++e) v[e] = e < each && first + 32 * e < n ? ids[first + 32 * e] : 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const bool in = e < each && first + 32 * e < n;
+        id[e] = in ? eo_id(v[e], V, padding, status) : -1;
+        tok[e] = first + 32 * e;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const bool in = e < each && first + 32 * e < n;
+        id[e] = in ? __ldcg(id_in + first + 32 * e) : -1;
+        tok[e] = in ? __ldcg(tok_in + first + 32 * e) : 0;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) in_warp[w][tid] = 0;
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const int i = first + 32 * e;
-      if (i - lane >= n) break;
-      id[e] = i < n ? id_at[from][i] : -1;
-      tok[e] = i < n ? tok_at[from][i] : 0;
-      const int digit = id[e] < 0 ? BINS : id[e] >> shift & ((1 << bits) - 1);
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      rank[e] = digit < BINS ? in_warp[warp][digit] + __popc(same & ((1u << lane) - 1)) : 0;
+      if (e >= each) break;
+      const int digit = id[e] >> shift & (BINS - 1) & ((1 << bits) - 1);
+      const uint32_t same = same_digit(digit, id[e] >= 0, bits);
+      rank[e] = in_warp[warp][digit] + __popc(same & ((1u << lane) - 1));
       __syncwarp();
-      if (digit < BINS && same >> lane == 1) in_warp[warp][digit] += __popc(same);             // (the last of them)
+      if (id[e] >= 0 && same >> lane == 1) in_warp[warp][digit] += __popc(same);               // (the last of them)
       __syncwarp();
     }
     __syncthreads();
-    {                                                              // SHARE threads a digit, each WARPS / SHARE warps' counts
-      const int digit = tid / SHARE, part = tid % SHARE;
-      int sum = 0;
+    int sum = 0;
 #pragma unroll
-      for (int w = 0; w < WARPS / SHARE; ++w) sum += in_warp[part * (WARPS / SHARE) + w][digit];
-      int upto = sum;
+    for (int w = 0; w < WARPS; ++w) { const int v = in_warp[w][tid]; in_warp[w][tid] = (unsigned short)sum; sum += v; }
+    count[tid] = sum;
+    cluster.sync();
+    int total = 0, before = 0;
 #pragma unroll
-      for (int o = 1; o < SHARE; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (part >= o) upto += v; }
-      int at = upto - sum;
-#pragma unroll
-      for (int w = 0; w < WARPS / SHARE; ++w) {
-        unsigned short& c = in_warp[part * (WARPS / SHARE) + w][digit];
-        const int v = c;
-        c = (unsigned short)at;
-        at += v;
-      }
-      if (part == SHARE - 1) base[digit] = upto;
+    for (int c = 0; c < ONE_CTAS; ++c) {
+      const int v = cluster.map_shared_rank(count, c)[tid];
+      total += v;
+      before += c < rank_in ? v : 0;
     }
+    base[tid] = sums_before(total, warp_total) + before;
     __syncthreads();
-    int v = 0, total = 0;
-    if (tid < BINS) {
-      total = v = base[tid];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += u; }
-      if (lane == 31) warp_total[warp] = v;
-    }
-    __syncthreads();
-    if (tid < BINS) {
-      int at = v - total;
-      for (int w = 0; w < warp; ++w) at += warp_total[w];
-      base[tid] = at;
-    }
-    __syncthreads();
-    int *id_out = pass + 1 < passes ? id_at[from ^ 1] : S.id, *tok_out = pass + 1 < passes ? tok_at[from ^ 1] : S.tok;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
       if (id[e] < 0) continue;
@@ -232,7 +258,7 @@ embedding_sort_kernel(const int64_t* __restrict__ ids, int n, int V, long long p
       id_out[at] = id[e];
       tok_out[at] = tok[e];
     }
-    __syncthreads();
+    cluster.sync();                                                  // (every CTA's places are written, its counts read)
   }
 }
 
@@ -247,8 +273,14 @@ embedding_count_kernel(const int64_t* __restrict__ ids, int n, int V, long long 
   if (blockIdx.x == 0 && tid == 0) *S.join_count = 0;
   __syncthreads();
   const int begin = blockIdx.x * span, end = min(begin + span, n);
-#pragma unroll 8
-  for (int i = begin + tid; i < end; i += SORT_THREADS) atomicAdd(&count[eo_id(ids[i], V, padding, status) & (bins - 1)], 1);
+  for (int i0 = begin + tid; i0 < end; i0 += 8 * SORT_THREADS) {
+    int64_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = i0 + e * SORT_THREADS < end ? ids[i0 + e * SORT_THREADS] : 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i0 + e * SORT_THREADS < end) atomicAdd(&count[eo_id(v[e], V, padding, status) & (bins - 1)], 1);
+  }
   __syncthreads();
   for (int b = tid; b < bins; b += SORT_THREADS) {
     S.hist[blockIdx.x * bins + b] = count[b];
@@ -285,13 +317,7 @@ embedding_place_kernel(const int64_t* __restrict__ ids, const int* __restrict__ 
     int sum = 0;
 #pragma unroll
     for (int u = 0; u < BINS_EACH; ++u) sum += total[u];
-    int upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
-    if (lane == 31) warp_total[warp] = upto;
-    __syncthreads();
-    int at = upto - sum;
-    for (int w = 0; w < warp; ++w) at += warp_total[w];
+    int at = sums_before(sum, warp_total);
     for (int u = 0; u < each; ++u) {
       const int b = tid * each + u;
       if (b < bins) base[b] = at + before[u];
@@ -312,11 +338,11 @@ embedding_place_kernel(const int64_t* __restrict__ ids, const int* __restrict__ 
     }
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const int digit = id[e] < 0 ? bins : id[e] >> shift & (bins - 1);
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      rank[e] = digit < bins ? in_warp[warp][digit] + __popc(same & ((1u << lane) - 1)) : 0;
+      const int digit = id[e] >> shift & (bins - 1);
+      const uint32_t same = same_digit(digit, id[e] >= 0, bits);
+      rank[e] = in_warp[warp][digit] + __popc(same & ((1u << lane) - 1));
       __syncwarp();
-      if (digit < bins && (same >> lane) == 1) in_warp[warp][digit] += __popc(same);           // (the last of them)
+      if (id[e] >= 0 && same >> lane == 1) in_warp[warp][digit] += __popc(same);           // (the last of them)
       __syncwarp();
     }
     __syncthreads();
@@ -444,11 +470,10 @@ embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __re
   rte::after_previous_grid();
   __shared__ float sum[JOIN_WARPS][JOIN_COLUMNS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int tiles = (d + JOIN_COLUMNS - 1) / JOIN_COLUMNS;
-  const long long jobs = (long long)*S.join_count * tiles;
-  for (long long job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const int2 join = S.joins[job / tiles];
-    const int r = join.x, v = join.y, c0 = int(job % tiles) * JOIN_COLUMNS;
+  const int joins = *S.join_count;
+  for (int j = blockIdx.x; j < joins; j += gridDim.x) {
+    const int2 join = S.joins[j];
+    const int r = join.x, v = join.y;
     // how many ranges behind r + 1 begin with the id: leaps of 1024, 32 and one range, a lane each, asked for at once
     const auto begins = [&](long long q) { const long long at = (r + 1 + q) * (long long)range; return at < n && S.id[at] == v; };
     int m = 0;
@@ -465,22 +490,26 @@ embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __re
     if (m > 0) near = begins(m + lane + 1);
     m += __popc(__ballot_sync(0xffffffffu, near)) + 1;             // r + 1 .. r + m
     const int first = int((long long)m * warp / JOIN_WARPS), last = int((long long)m * (warp + 1) / JOIN_WARPS);
-    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c0 = blockIdx.y * JOIN_COLUMNS; c0 < d; c0 += gridDim.y * JOIN_COLUMNS) {
+      const bool mine = tid < JOIN_COLUMNS && c0 + tid < d;
+      const float begun = mine ? S.part[((size_t)r * 2 + 1) * d + c0 + tid] : 0.f;
+      float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int q = first; q < last; ++q)
+      for (int q = first; q < last; ++q)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c0 + lane + 32 * u < d) a[u] += S.part[(size_t)(r + 1 + q) * 2 * d + c0 + lane + 32 * u];
+        for (int u = 0; u < 4; ++u)
+          if (c0 + lane + 32 * u < d) a[u] += S.part[(size_t)(r + 1 + q) * 2 * d + c0 + lane + 32 * u];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) sum[warp][lane + 32 * u] = a[u];
-    __syncthreads();
-    if (tid < JOIN_COLUMNS && c0 + tid < d) {
-      float s = S.part[((size_t)r * 2 + 1) * d + c0 + tid];
+      for (int u = 0; u < 4; ++u) sum[warp][lane + 32 * u] = a[u];
+      __syncthreads();
+      if (mine) {
+        float s = begun;
 #pragma unroll
-      for (int w = 0; w < JOIN_WARPS; ++w) s += sum[w][tid];
-      dtable[(long long)v * d + c0 + tid] = (T)(s * scale);
+        for (int w = 0; w < JOIN_WARPS; ++w) s += sum[w][tid];
+        dtable[(long long)v * d + c0 + tid] = (T)(s * scale);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -506,31 +535,34 @@ void launch_sum(const void* dy, const EoScratch& s, int n, int V, int d, float s
   const int range_ctas = rte::ceil_div(ranges, 128 / tpr);
   const dim3 grid(range_ctas + (filled ? 0 : rte::ceil_div(V, ZERO_ROWS)), (unsigned)min(rte::ceil_div(pieces, tpr), 64));
   rte::launch(embedding_sum_kernel<T, BYTES>, grid, 128, 0, st, static_cast<const T*>(dy), s, n, V, pieces, tpr, range, d, scale, static_cast<T*>(dtable), range_ctas);
-  if (ranges > 1)
-    rte::launch(embedding_join_kernel<T>, min(rte::ceil_div64((long long)(ranges - 1) * d, JOIN_COLUMNS), 148LL * 8), 32 * JOIN_WARPS, 0, st, s, n, range, d, scale,
-                static_cast<T*>(dtable));
+  if (ranges > 2) {                                                // (an id that is joined fills a range between two others)
+    const int tiles = min(rte::ceil_div(d, JOIN_COLUMNS), 64);
+    rte::launch(embedding_join_kernel<T>, dim3(min(ranges - 2, rte::ceil_div(148 * 8, tiles)), tiles), 32 * JOIN_WARPS, 0, st, s, n, range, d, scale, static_cast<T*>(dtable));
+  }
 }
 
-// id and tok sorted; `table` (NULL: not) filled with zeros on the way.
+// id and tok sorted; `table` (NULL: not) filled with zeros on the way, by FILL_CTAS CTAs in each launch (33333 x 770 fp32 of 50257, the whole
+// gradient, 1 | 2 | 7 | 16 of them per SM: 91 | 78 | 72 | 70 us), a pass's share twice that of the count, which is done sooner.
+constexpr int FILL_CTAS = 16 * 148;
 void launch_sort(const int64_t* ids, int n, int V, long long padding, const EoScratch& s, char* table, long long table_bytes, int* status, cudaStream_t st) {
   const bool one = n <= SORT_ONE;
   const Digits dg = digits_of(V, one ? ONE_BITS : SORT_BITS);
-  const int launches = one ? 1 : 1 + dg.passes, fills = table ? (one ? 147 : 2 * 148) : 0;
-  const long long part = table ? rte::ceil_div64(rte::ceil_div64(table_bytes, launches), 256) * 256 : 0;
-  auto slice = [&](int i) { const long long at = min(i * part, table_bytes); return Fill{table + at, min(part, table_bytes - at)}; };
+  const int fills = table ? FILL_CTAS : 0, shares = one ? 1 : 1 + 2 * dg.passes;
+  const long long share = table ? rte::ceil_div64(rte::ceil_div64(table_bytes, shares), 256) * 256 : 0;
+  auto slice = [&](int from, int to) { const long long at = min(from * share, table_bytes); return Fill{table + at, min(to * share, table_bytes) - at}; };
   if (one) {
-    rte::launch(embedding_sort_kernel, 1 + fills, ONE_THREADS, one_bytes(n), st, ids, n, V, padding, s, dg.passes, dg.bits, slice(0), status);
+    rte::launch(embedding_sort_kernel, ONE_CTAS + fills, SORT_THREADS, 0, st, ids, n, V, padding, s, dg.passes, dg.bits, slice(0, 1), status);
     return;
   }
   const int span = sort_span(n), ctas = rte::ceil_div(n, span);
-  rte::launch(embedding_count_kernel, ctas + fills, SORT_THREADS, 0, st, ids, n, V, padding, s, dg.passes, dg.bits, span, ctas, slice(0), status);
+  rte::launch(embedding_count_kernel, ctas + fills, SORT_THREADS, 0, st, ids, n, V, padding, s, dg.passes, dg.bits, span, ctas, slice(0, 1), status);
   const int *id = nullptr, *tok = nullptr;
   for (int p = 0; p < dg.passes; ++p) {
     const bool to_first = (dg.passes - 1 - p) % 2 == 0;
     int *id_out = to_first ? s.id : s.id2, *tok_out = to_first ? s.tok : s.tok2;
     const auto place = sort_each(n) == 2 ? embedding_place_kernel<2> : sort_each(n) == 4 ? embedding_place_kernel<4> : embedding_place_kernel<8>;
     rte::launch(place, ctas + fills, SORT_THREADS, 0, st, ids, id, tok, id_out, tok_out, s.hist, n, V, padding, p, dg.passes, dg.bits, span, ctas,
-                slice(1 + p));
+                slice(1 + 2 * p, 3 + 2 * p));
     id = id_out;
     tok = tok_out;
   }
@@ -584,8 +616,6 @@ extern "C" int rte_embedding_bwd(const int64_t* ids, int64_t n, const void* dy, 
   if (type == RTE_TYPE_F32 && bytes < 4) return RTE_ERR_ALIGNMENT;
   EoScratch s;
   eo_layout(static_cast<char*>(scratch), n, d, &s);
-  if (n <= SORT_ONE && cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one_bytes(SORT_ONE)) != cudaSuccess)
-    return RTE_ERR_LAUNCH;
   // Rows that no token names: with fewer tokens than rows the whole table is filled beside the sort, and the named rows are written again.
   const bool fill_ahead = n <= V;
   launch_sort(ids, (int)n, V, padding_idx, s, fill_ahead ? static_cast<char*>(dtable) : nullptr, (long long)V * d * (type == RTE_TYPE_F32 ? 4 : 2), status, ST(stream));
