@@ -306,7 +306,7 @@ int rte_ce_gradient(const void* logits, int32_t f32, int32_t ldl, const int64_t*
  * rte_token_logprobs_fwd: logprob f32 [rows] of tokens[row], entropy f32 [rows], the top_k largest as top_logprobs f32 / top_ids
  *   int64 [rows, top_k] in descending order (equal logits: lower column first; NaN above all).  A row whose token is ignore_index (or
  *   out of range, which sets status) is not read: zeros, ids -1.  A row of nothing but -inf: log probabilities -inf, entropy 0.
- *   row_stats f32 [rows, 2] is kept for backward.
+ *   row_stats f32 [rows, 2] is kept for backward (NULL: none follows; so for distillation).
  * rte_token_logprobs_bwd: dlogits [rows, V] contiguous, of `type`, from the gradients of logprob, entropy and top_logprobs (NULL: none);
  *   zeros in rows without a token or a finite logit.
  * rte_distill_topk_fwd: loss f32 [rows] = temperature^2 * KL(teacher || softmax(logits / temperature)).  The teacher's row is a list of

@@ -516,27 +516,39 @@ struct Rows {                                 // [..., V] as rows of one stride:
 // The kernels take the number of rows as an int32.
 void count_fits(int64_t n, const char* what) { TORCH_CHECK_VALUE(n < (int64_t(1) << 31), what, ": ", n, " rows in one call"); }
 Tensor grad_f32(const Tensor& g) { return g.defined() ? g.to(F32).contiguous() : Tensor(); }
+// Where nothing asks for a gradient an operator is its launches alone: no node (3 us of the host's time) and nothing kept for backward.
+bool differentiable(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 struct TokenLogprobs : Function<TokenLogprobs> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index) {
+  struct Out { Tensor tok, logprob, entropy, top_lp, top_ids; };
+  static Out run(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index, Tensor* stats) {
     Dev dev(logits);
     const Rows x(logits);
     count_fits(x.rows, "k_token_logprobs");
-    const Tensor tok = tokens.to(torch::kInt64).contiguous();
+    Out o;
+    o.tok = tokens.to(torch::kInt64).contiguous();
     std::vector<int64_t> top(tokens.sizes().begin(), tokens.sizes().end());
     top.push_back(top_k);
-    const Tensor logprob = empty_as(tok, F32), entropy = empty_as(tok, F32), stats = empty({x.rows, 2}, F32, logits);
-    const Tensor top_lp = at::empty(top, tok.options().dtype(F32)), top_ids = at::empty(top, tok.options());
+    o.logprob = empty_as(o.tok, F32);
+    o.entropy = empty_as(o.tok, F32);
+    if (stats) *stats = empty({x.rows, 2}, F32, logits);
+    o.top_lp = at::empty(top, o.tok.options().dtype(F32));
+    o.top_ids = at::empty(top, o.tok.options());
     if (x.rows > 0)
-      check(rte_token_logprobs_fwd(ptr(x.t), type_of(x.t), x.ld, tok.data_ptr<int64_t>(), ignore_index, temperature, top_k, f32(logprob), f32(entropy), f32(top_lp),
-                                   top_ids.data_ptr<int64_t>(), f32(stats), x.rows, x.V, dev.status, dev.st),
+      check(rte_token_logprobs_fwd(ptr(x.t), type_of(x.t), x.ld, o.tok.data_ptr<int64_t>(), ignore_index, temperature, top_k, f32(o.logprob), f32(o.entropy), f32(o.top_lp),
+                                   o.top_ids.data_ptr<int64_t>(), stats ? f32(*stats) : nullptr, x.rows, x.V, dev.status, dev.st),
             "rte_token_logprobs_fwd");
+    return o;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index) {
+    Tensor stats;
+    const Out o = run(logits, tokens, top_k, temperature, ignore_index, &stats);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, tok, stats, entropy, top_ids});
-    ctx->mark_non_differentiable({top_ids});
+    ctx->save_for_backward({logits, o.tok, stats, o.entropy, o.top_ids});
+    ctx->mark_non_differentiable({o.top_ids});
     ctx->saved_data["top_k"] = top_k;
     ctx->saved_data["temperature"] = temperature;
-    return {logprob, entropy, top_lp, top_ids};
+    return {o.logprob, o.entropy, o.top_lp, o.top_ids};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
@@ -553,22 +565,30 @@ struct TokenLogprobs : Function<TokenLogprobs> {
   }
 };
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index) {
+  if (!differentiable(logits)) {
+    const auto o = TokenLogprobs::run(logits, tokens, top_k, temperature, ignore_index, nullptr);
+    return {o.logprob, o.entropy, o.top_lp, o.top_ids};
+  }
   auto out = TokenLogprobs::apply(logits, tokens, top_k, temperature, ignore_index);
   return {out[0], out[1], out[2], out[3]};
 }
 
 struct DistillTopk : Function<DistillTopk> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature, bool tail) {
+  static Tensor run(const Tensor& logits, const Tensor& t, const Tensor& id, double temperature, bool tail, Tensor* stats) {
     Dev dev(logits);
     const Rows x(logits);
     count_fits(x.rows, "k_distill_topk");
-    const auto k = ids.size(-1);
-    const Tensor t = teacher.to(F32).contiguous(), id = ids.to(torch::kInt64).contiguous();
-    const Tensor loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), t.options()), stats = empty({x.rows, 8}, F32, logits);
+    const Tensor loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), t.options());
+    if (stats) *stats = empty({x.rows, 8}, F32, logits);
     if (x.rows > 0)
-      check(rte_distill_topk_fwd(ptr(x.t), type_of(x.t), x.ld, f32(t), id.data_ptr<int64_t>(), k, temperature, tail, f32(loss), f32(stats), x.rows, x.V, dev.status,
-                                 dev.st),
+      check(rte_distill_topk_fwd(ptr(x.t), type_of(x.t), x.ld, f32(t), id.data_ptr<int64_t>(), id.size(-1), temperature, tail, f32(loss),
+                                 stats ? f32(*stats) : nullptr, x.rows, x.V, dev.status, dev.st),
             "rte_distill_topk_fwd");
+    return loss;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& t, const Tensor& id, double temperature, bool tail) {
+    Tensor stats;
+    const Tensor loss = run(logits, t, id, temperature, tail, &stats);
     ctx->save_for_backward({logits, t, id, stats});
     ctx->saved_data["temperature"] = temperature;
     return {loss};
@@ -586,19 +606,25 @@ struct DistillTopk : Function<DistillTopk> {
   }
 };
 Tensor distill_topk(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature, bool tail) {
-  return DistillTopk::apply(logits, teacher.detach(), ids, temperature, tail)[0];
+  const Tensor t = teacher.detach().to(F32).contiguous(), id = ids.to(torch::kInt64).contiguous();
+  return differentiable(logits) ? DistillTopk::apply(logits, t, id, temperature, tail)[0] : DistillTopk::run(logits, t, id, temperature, tail, nullptr);
 }
 
 // --------------------------------------------------------------------------- embedding
 struct Embedding : Function<Embedding> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) {
+  static Tensor run(const Tensor& id, const Tensor& weight, double scale) {
     Dev dev(weight);
-    const Tensor id = ids.to(torch::kInt64).contiguous(), w = weight.contiguous();
+    const Tensor w = weight.contiguous();
     const auto n = id.numel(), V = w.size(0), d = w.size(1);
-    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+    std::vector<int64_t> shape(id.sizes().begin(), id.sizes().end());
     shape.push_back(d);
     const Tensor out = at::empty(shape, w.options());
     if (n > 0) check(rte_embedding_fwd(id.data_ptr<int64_t>(), n, ptr(w), type_of(w), V, d, scale, ptr(out), dev.status, dev.st), "rte_embedding_fwd");
+    return out;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& id, const Tensor& weight, double scale, int64_t padding_idx) {
+    const Tensor out = run(id, weight, scale);
+    const auto V = weight.size(0), d = weight.size(1);
     ctx->save_for_backward({id});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["dims"] = std::vector<int64_t>{V, d, padding_idx};
@@ -618,7 +644,10 @@ struct Embedding : Function<Embedding> {
     return {Tensor(), dw, Tensor(), Tensor()};
   }
 };
-Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) { return Embedding::apply(ids, weight, scale, padding_idx)[0]; }
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) {
+  const Tensor id = ids.to(torch::kInt64).contiguous();
+  return differentiable(weight) ? Embedding::apply(id, weight, scale, padding_idx)[0] : Embedding::run(id, weight, scale);
+}
 
 // --------------------------------------------------------------------------- packed SwiGLU FFN
 struct PackedFfn : Function<PackedFfn> {

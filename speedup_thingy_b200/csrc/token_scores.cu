@@ -552,7 +552,11 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   if (tok < 0 || tok >= V) {
     if (rank == 0) {
       if (tok != ignore && status && tid == 0) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
-      if (tid == 0) { logprob[row_at] = 0.f; entropy[row_at] = 0.f; stats[row_at] = make_float2(0.f, -INFINITY); }
+      if (tid == 0) {
+        logprob[row_at] = 0.f;
+        entropy[row_at] = 0.f;
+        if (stats) stats[row_at] = make_float2(0.f, -INFINITY);
+      }
       for (int i = tid; i < k; i += NT) { top_lp[row_at * k + i] = 0.f; top_ids[row_at * k + i] = -1; }
     }
     return;
@@ -621,7 +625,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
     logprob[row_at] = log_p(target);
     // H = ln s - sum t 2^t / s, relative to the same R
     entropy[row_at] = none ? 0.f : LN2 * (log2f(a.s) - a.e / a.s);
-    stats[row_at] = make_float2(a.top, none ? -INFINITY : log2f(a.s));
+    if (stats) stats[row_at] = make_float2(a.top, none ? -INFINITY : log2f(a.s));
   }
   for (int i = tid; i < n; i += NT) {                            // the list's order: how many keys come before
     const unsigned long long key = list[i];
@@ -693,7 +697,10 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   }
   any = __syncthreads_or(any);
   if (!any) {                                                    // (the same in all CTAs of the cluster)
-    if (rank == 0 && tid == 0) { loss[row_at] = 0.f; stats[row_at * 2] = stats[row_at * 2 + 1] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    if (rank == 0 && tid == 0) {
+      loss[row_at] = 0.f;
+      if (stats) stats[row_at * 2] = stats[row_at * 2 + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     return;
   }
   const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
@@ -779,6 +786,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
     P = M * P - r;                                               // (what the others' gradient is in proportion to)
   }
   loss[row_at] = float(L * temp * temp);
+  if (!stats) return;
   // 2^-l2 of a sum relative to the rounded reference that backward forms again: the others' among themselves, and the row's
   const bool others = a.s != 0.f;
   const double l2 = ln_s * LOG2E + (far(top, c) ? 0. : (double)top * c - reference(top, c));
@@ -986,7 +994,7 @@ float log2_scale(float temperature) { return (float)(LOG2E / temperature); }
 extern "C" int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t ldl, const int64_t* tokens, int64_t ignore_index, float temperature, int32_t top_k,
                                       float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, float* row_stats, int32_t rows, int32_t V, int32_t* status,
                                       rte_stream_t stream) {
-  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && tokens && logprob && entropy && row_stats && temperature_ok(temperature));
+  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && tokens && logprob && entropy && temperature_ok(temperature));
   RTE_CHECK_ARG(top_k >= 0 && top_k <= V && top_k <= TS_MAX_LIST && (top_k == 0 || (top_logprobs && top_ids)));
   if (!on_element(logits, type) || reinterpret_cast<uintptr_t>(row_stats) % 8) return RTE_ERR_ALIGNMENT;
   const int pieces = pieces_of(logits, type, ldl, V);
@@ -1027,7 +1035,7 @@ extern "C" int rte_token_logprobs_bwd(const void* logits, int32_t type, int64_t 
 
 extern "C" int rte_distill_topk_fwd(const void* logits, int32_t type, int64_t ldl, const float* teacher, const int64_t* ids, int32_t k, float temperature, int32_t tail,
                                     float* loss, float* row_stats, int32_t rows, int32_t V, int32_t* status, rte_stream_t stream) {
-  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && teacher && ids && loss && row_stats && temperature_ok(temperature));
+  RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && teacher && ids && loss && temperature_ok(temperature));
   RTE_CHECK_ARG(k > 0 && k <= TS_MAX_LIST);
   if (!on_element(logits, type) || reinterpret_cast<uintptr_t>(row_stats) % 16) return RTE_ERR_ALIGNMENT;
   const int pieces = pieces_of(logits, type, ldl, V);

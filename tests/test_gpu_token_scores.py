@@ -495,6 +495,22 @@ def test_same_bits_every_time_on_a_side_stream_and_from_a_graph(rows, V):
     K._ops_for(x).check_status()
 
 
+@pytest.mark.parametrize("rows, V", [(3, 70), (5, 40000), (700, 9000)])
+def test_without_a_gradient_the_same_results(rows, V):
+    x = made(rows, V, torch.bfloat16)
+    tokens = torch.randint(0, V, (rows,), device=DEV)
+    tokens[0] = -100
+    t, ids = a_teacher(x, 8, 1.0)
+    ids[1] = -1
+    leaf = x.clone().requires_grad_()
+    for a, b in zip(K.k_token_logprobs(x, tokens, top_k=5), K.k_token_logprobs(leaf, tokens, top_k=5)):
+        assert torch.equal(a, b) and not a.requires_grad
+    for tail in (False, True):
+        assert torch.equal(K.k_distill_topk(x, t, ids, tail=tail), K.k_distill_topk(leaf, t, ids, tail=tail))
+    with torch.no_grad():
+        assert not K.k_token_logprobs(leaf, tokens).logprob.requires_grad and not K.k_distill_topk(leaf, t, ids).requires_grad
+
+
 def test_logits_changed_in_place_are_refused_by_backward():
     x = made(2, 64, torch.float32).requires_grad_()
     y = x * 1.0

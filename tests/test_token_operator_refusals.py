@@ -72,12 +72,12 @@ EMBED_BWD = dict(ids=P, n=4, dy=P, type=A.TYPE_BF16, V=16, d=8, scale=1.0, paddi
 
 
 @pytest.mark.parametrize("name, args, change, code", [
-    *[("rte_token_logprobs_fwd", SCORES, {k: None}, BAD) for k in ("logits", "tokens", "logprob", "entropy", "top", "ids", "stats")],
+    *[("rte_token_logprobs_fwd", SCORES, {k: None}, BAD) for k in ("logits", "tokens", "logprob", "entropy", "top", "ids")],
     *[("rte_token_logprobs_fwd", SCORES, c, BAD) for c in ({"type": 3}, {"type": -1}, {"ldl": -1}, {"temperature": 0.0}, {"temperature": float("nan")}, {"k": -1},
                                                          {"k": 65}, {"k": 257, "V": 1000}, {"rows": 0}, {"rows": -5}, {"V": 0})],
     *[("rte_token_logprobs_bwd", SCORES_BWD, {k: None}, BAD) for k in ("logits", "tokens", "ids", "stats", "entropy", "dlogits")],
     *[("rte_token_logprobs_bwd", SCORES_BWD, c, BAD) for c in ({"type": 3}, {"ldl": -1}, {"temperature": -1.0}, {"k": 65}, {"rows": 0}, {"V": 0})],
-    *[("rte_distill_topk_fwd", DISTILL, {k: None}, BAD) for k in ("logits", "teacher", "ids", "loss", "stats")],
+    *[("rte_distill_topk_fwd", DISTILL, {k: None}, BAD) for k in ("logits", "teacher", "ids", "loss")],
     *[("rte_distill_topk_fwd", DISTILL, c, BAD) for c in ({"type": 3}, {"ldl": -1}, {"temperature": 0.0}, {"k": 0}, {"k": 257}, {"rows": 0}, {"V": 0})],
     ("rte_distill_topk_fwd", DISTILL, {"stats": C.c_void_p(4100)}, ALIGN),
     *[("rte_distill_topk_bwd", DISTILL_BWD, {k: None}, BAD) for k in ("logits", "teacher", "ids", "stats", "dloss", "dlogits")],
