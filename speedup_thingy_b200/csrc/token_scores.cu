@@ -20,8 +20,8 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int TS_MAX_LIST = RTE_TOKEN_LIST_MAX;
-// Forward's CTAs on an SM: 24 to 32 warps are in flight, a thread has 85, 48 or 64 registers.
-__host__ __device__ constexpr int min_ctas(int nt) { return nt == 32 ? 24 : nt == 128 ? 10 : 4; }
+// Forward's CTAs on an SM: 24 to 40 warps are in flight, a thread has 80, 48 or 64 registers.
+__host__ __device__ constexpr int min_ctas(int nt, int u) { return nt == 32 ? 24 : nt == 256 ? 4 : u == 4 ? 10 : 8; }
 constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.44269504088896340736, LN2_D = 0.693147180559945309417;
@@ -236,7 +236,7 @@ struct TopK {                                            // in shared memory, si
   __device__ __forceinline__ unsigned long long* column_list() const { return piece + most(k); }
 };
 // Tiles whose pieces' maxima are kept before they are looked through: 512, 1024 and 2048 pieces.
-__host__ __device__ constexpr int round_tiles(int nt) { return nt == 256 ? 1 : nt == 128 ? 2 : 4; }
+__host__ __device__ constexpr int round_tiles(int nt, int u) { return nt == 32 ? 4 : nt == 128 && u == 4 ? 2 : 1; }
 
 template <int NT> __device__ __forceinline__ void sync() { if (NT == 32) __syncwarp(); else __syncthreads(); }
 template <int NT> __device__ __forceinline__ int sync_or(int v) { return NT == 32 ? __any_sync(0xffffffffu, v) : __syncthreads_or(v); }
@@ -444,7 +444,7 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
   constexpr int N = Vec<T>::N, TILE = NT * U;
   const int tid = threadIdx.x;
   Sums a = no_sums(c);
-  constexpr int ROUND = round_tiles(NT);
+  constexpr int ROUND = round_tiles(NT, U);
   int in_round = 0;
   float round_top = 0.f;
   for (int tile = begin; tile < end; tile += TILE) {
@@ -538,12 +538,12 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
 // ---------------------------------------------------------------- forward
 // A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.
 template <typename T, int NT, int U, bool TOP>
-__global__ void __launch_bounds__(NT, min_ctas(NT))
+__global__ void __launch_bounds__(NT, min_ctas(NT, U))
 token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, float inv_t, int k, float* __restrict__ logprob,
                       float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids, float2* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
   extern __shared__ __align__(16) unsigned char dyn[];
-  TopK top(dyn, k, NT, NT * U * round_tiles(NT));                                     // (there is none without TOP)
+  TopK top(dyn, k, NT, NT * U * round_tiles(NT, U));                                     // (there is none without TOP)
   __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
   __shared__ Sums mine;
   const long long row_at = blockIdx.x / C;
@@ -669,7 +669,7 @@ __device__ __forceinline__ float block_max_float(float v, float* red) {
 // stats of a row, eight floats: for the columns outside the list (all, without TAIL) their largest logit, log2 of their sum and what
 // their share of it is multiplied by; M (0: no gradient); the list's max, ln of its sum; the row's largest logit, log2 of its sum
 template <typename T, int NT, int U, bool TAIL>
-__global__ void __launch_bounds__(NT, min_ctas(NT))
+__global__ void __launch_bounds__(NT, min_ctas(NT, U))
 distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, double temp,
                     float* __restrict__ loss, float4* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
@@ -942,10 +942,12 @@ void launch_cluster(K kernel, long long ctas, int nt, size_t smem, int C, cudaSt
   (void)cudaLaunchKernelEx(&cfg, kernel, args...);               // (an error stays pending for RTE_LAUNCH_CHECK)
 }
 
-// CTAs per row: as many (up to 8) as bring two CTAs to every SM, with a tile of pieces each.
-int cluster_of(long long rows, int pieces, int tile) {
+// CTAs per row: as many (up to 8) as come to ten on an SM, with a tile of pieces each; to four where their lists have to be joined too.
+// us, 1 | 2 | 4 | 8 per row: 300 x 50257 bf16 13.1 | 12.4 | 10.3 | 15.6, 700 x 50257 21 | 15.6 | 18.8 | 30; with lists 61 x 131072 fp32
+// 42 | 29 | 20 | 19, 1000 x 32768 bf16 31 | 38 | 55 | 103.
+int cluster_of(long long rows, int pieces, int tile, bool lists) {
   int C = 1;
-  while (C < 8 && rows * C < 2 * 148 && pieces > C * tile) C *= 2;
+  while (C < 8 && rows * C * 2 <= (lists ? 4 : 10) * 148 && pieces > C * tile) C *= 2;
   return C;
 }
 // The most pieces a row of V columns has: one more where rows do not all start on 16 bytes.
@@ -957,27 +959,29 @@ int pieces_of(const void* x, int type, long long ld, int V) {
 
 // A row of at most one tile of 32 or 128 threads is one CTA of them; longer ones are walked by 256.
 // Forward, who walks a row.  Many short rows: a warp each (us, 8192 x 2048 bf16, warp | 128 threads: 11.0 | 20, with 32 alternatives 39 | 60;
-// 256 rows of it: 6.2 | 4.8).  Many long ones: 128 threads (8192 x 32768 bf16, warp | 128 | 256 | 512: 119 | 97 | 105 | 151).  Few long ones,
-// where latency counts: 256 threads, eight loads each (1 x 50257 with 20 alternatives, 128 x 4 | 256 x 4 | 256 x 8: 12.8 | 10.7 | 9.2).
+// 256 rows of it: 6.2 | 4.8).  Many long ones: 128 threads (8192 x 32768 bf16, warp | 128 | 256 | 512: 119 | 97 | 105 | 151), eight loads each for
+// scores, four for distillation, which has more to keep (2000 x 131072 with 64 alternatives, 4 | 8: 133 | 118; 8192 x 32768 distilled 127 | 134).
+// Few long ones, where latency counts: 256 threads, eight loads each (1 x 50257 with 20 alternatives, 128 x 4 | 256 x 4 | 256 x 8: 12.8 | 10.7 | 9.2).
 constexpr int MANY_SHORT = 20 * 148, MANY_LONG = 2 * 148;
-#define FORWARD(T, rows, pieces, CALL)                                              \
-  do {                                                                              \
-    if (pieces <= 128 || (pieces <= 512 && rows >= MANY_SHORT)) CALL(T, 32, 4);     \
-    else if (pieces <= 512 || rows >= MANY_LONG) CALL(T, 128, 4);                   \
-    else CALL(T, 256, 8);                                                           \
+#define FORWARD(T, rows, pieces, LOADS, CALL) \
+  do { \
+    if (pieces <= 128 || (pieces <= 512 && rows >= MANY_SHORT)) CALL(T, 32, 4); \
+    else if (pieces <= 512) CALL(T, 128, 4); \
+    else if (rows >= MANY_LONG) CALL(T, 128, LOADS); \
+    else CALL(T, 256, 8); \
   } while (0)
 // Backward: CTAs of a warp for rows that it covers, of 128 threads for others, all 2048 of an SM (8192 x 32768 bf16, 128 | 256 threads:
 // 163 | 174; 8192 x 2048, warp | 128: 17.9 | 13.7).
-#define BACKWARD(T, rows, pieces, CALL)     \
-  do {                                      \
-    if (pieces <= 128) CALL(T, 32, 4);      \
-    else CALL(T, 128, 4);                   \
+#define BACKWARD(T, rows, pieces, LOADS, CALL) \
+  do { \
+    if (pieces <= 128) CALL(T, 32, 4); \
+    else CALL(T, 128, 4); \
   } while (0)
-#define BY_TYPE(type, WHICH, rows, pieces, CALL)                              \
-  do {                                                                        \
-    if (type == RTE_TYPE_BF16) WHICH(__nv_bfloat16, rows, pieces, CALL);      \
-    else if (type == RTE_TYPE_F16) WHICH(__half, rows, pieces, CALL);         \
-    else WHICH(float, rows, pieces, CALL);                                    \
+#define BY_TYPE(type, WHICH, rows, pieces, LOADS, CALL) \
+  do { \
+    if (type == RTE_TYPE_BF16) WHICH(__nv_bfloat16, rows, pieces, LOADS, CALL); \
+    else if (type == RTE_TYPE_F16) WHICH(__half, rows, pieces, LOADS, CALL); \
+    else WHICH(float, rows, pieces, LOADS, CALL); \
   } while (0)
 
 bool temperature_ok(float t) { return t >= MIN_T && t <= MAX_T; }
@@ -998,15 +1002,15 @@ extern "C" int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t 
   RTE_CHECK_ARG(top_k >= 0 && top_k <= V && top_k <= TS_MAX_LIST && (top_k == 0 || (top_logprobs && top_ids)));
   if (!on_element(logits, type) || reinterpret_cast<uintptr_t>(row_stats) % 8) return RTE_ERR_ALIGNMENT;
   const int pieces = pieces_of(logits, type, ldl, V);
-#define CALL(T, NT, U)                                                                                                                                       \
-  do {                                                                                                                                                       \
-    const int C = cluster_of(rows, pieces, NT * U);                                                                                                          \
-    launch_cluster(top_k > 0 ? token_logprobs_kernel<T, NT, U, true> : token_logprobs_kernel<T, NT, U, false>, (long long)rows * C, NT,                      \
-                   top_k > 0 ? TopK::shared_bytes(top_k, NT, NT * U * round_tiles(NT)) : 0, C, ST(stream), static_cast<const T*>(logits), (long long)ldl,                                         \
-                   tokens, (long long)ignore_index, log2_scale(temperature), 1.f / temperature, (int)top_k, logprob, entropy, top_logprobs,    \
-                   top_ids, reinterpret_cast<float2*>(row_stats), (int)V, C, status);                                                                        \
+#define CALL(T, NT, U) \
+  do { \
+    const int C = cluster_of(rows, pieces, NT * U, top_k > 0); \
+    launch_cluster(top_k > 0 ? token_logprobs_kernel<T, NT, U, true> : token_logprobs_kernel<T, NT, U, false>, (long long)rows * C, NT, \
+                   top_k > 0 ? TopK::shared_bytes(top_k, NT, NT * U * round_tiles(NT, U)) : 0, C, ST(stream), static_cast<const T*>(logits), (long long)ldl, \
+                   tokens, (long long)ignore_index, log2_scale(temperature), 1.f / temperature, (int)top_k, logprob, entropy, top_logprobs, \
+                   top_ids, reinterpret_cast<float2*>(row_stats), (int)V, C, status); \
   } while (0)
-  BY_TYPE(type, FORWARD, rows, pieces, CALL);
+  BY_TYPE(type, FORWARD, rows, pieces, 8, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -1019,15 +1023,15 @@ extern "C" int rte_token_logprobs_bwd(const void* logits, int32_t type, int64_t 
   RTE_CHECK_ARG(top_k >= 0 && top_k <= V && top_k <= TS_MAX_LIST && (!g_top || top_k == 0 || top_ids));
   if (!on_element(logits, type) || !on_element(dlogits, type) || reinterpret_cast<uintptr_t>(row_stats) % 8) return RTE_ERR_ALIGNMENT;
   const int pieces = pieces_of(logits, type, ldl, V);
-#define CALL(T, NT, U)                                                                                                                                        \
-  do {                                                                                                                                                        \
-    const int parts = rte::ceil_div(pieces, NT * U);                                                                                                          \
-    if ((long long)rows * parts > 0x7fffffff) return RTE_ERR_UNSUPPORTED;                                                                                      \
-    rte::launch(token_logprobs_bwd_kernel<T, NT, U>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, tokens, log2_scale(temperature),     \
+#define CALL(T, NT, U) \
+  do { \
+    const int parts = rte::ceil_div(pieces, NT * U); \
+    if ((long long)rows * parts > 0x7fffffff) return RTE_ERR_UNSUPPORTED; \
+    rte::launch(token_logprobs_bwd_kernel<T, NT, U>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, tokens, log2_scale(temperature), \
                 1.f / temperature, top_k, top_ids, reinterpret_cast<const float2*>(row_stats), entropy, g_logprob, g_entropy, g_top, static_cast<T*>(dlogits), V, \
-                parts);                                                                                                                                       \
+                parts); \
   } while (0)
-  BY_TYPE(type, BACKWARD, rows, pieces, CALL);
+  BY_TYPE(type, BACKWARD, rows, pieces, 4, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -1039,14 +1043,14 @@ extern "C" int rte_distill_topk_fwd(const void* logits, int32_t type, int64_t ld
   RTE_CHECK_ARG(k > 0 && k <= TS_MAX_LIST);
   if (!on_element(logits, type) || reinterpret_cast<uintptr_t>(row_stats) % 16) return RTE_ERR_ALIGNMENT;
   const int pieces = pieces_of(logits, type, ldl, V);
-#define CALL(T, NT, U)                                                                                                                                         \
-  do {                                                                                                                                                         \
-    const int C = cluster_of(rows, pieces, NT * U);                                                                                                            \
-    launch_cluster(tail ? distill_topk_kernel<T, NT, U, true> : distill_topk_kernel<T, NT, U, false>, (long long)rows * C, NT, 0, C, ST(stream),               \
-                   static_cast<const T*>(logits), (long long)ldl, teacher, ids, (int)k, log2_scale(temperature), (double)temperature, loss,                    \
-                   reinterpret_cast<float4*>(row_stats), (int)V, C, status);                                                                                   \
+#define CALL(T, NT, U) \
+  do { \
+    const int C = cluster_of(rows, pieces, NT * U, false); \
+    launch_cluster(tail ? distill_topk_kernel<T, NT, U, true> : distill_topk_kernel<T, NT, U, false>, (long long)rows * C, NT, 0, C, ST(stream), \
+                   static_cast<const T*>(logits), (long long)ldl, teacher, ids, (int)k, log2_scale(temperature), (double)temperature, loss, \
+                   reinterpret_cast<float4*>(row_stats), (int)V, C, status); \
   } while (0)
-  BY_TYPE(type, FORWARD, rows, pieces, CALL);
+  BY_TYPE(type, FORWARD, rows, pieces, 4, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
@@ -1058,14 +1062,14 @@ extern "C" int rte_distill_topk_bwd(const void* logits, int32_t type, int64_t ld
   RTE_CHECK_ARG(k > 0 && k <= TS_MAX_LIST);
   if (!on_element(logits, type) || !on_element(dlogits, type) || reinterpret_cast<uintptr_t>(row_stats) % 16) return RTE_ERR_ALIGNMENT;
   const int pieces = pieces_of(logits, type, ldl, V);
-#define CALL(T, NT, U)                                                                                                                                       \
-  do {                                                                                                                                                       \
-    const int parts = rte::ceil_div(pieces, NT * U);                                                                                                         \
-    if ((long long)rows * parts > 0x7fffffff) return RTE_ERR_UNSUPPORTED;                                                                                     \
+#define CALL(T, NT, U) \
+  do { \
+    const int parts = rte::ceil_div(pieces, NT * U); \
+    if ((long long)rows * parts > 0x7fffffff) return RTE_ERR_UNSUPPORTED; \
     rte::launch(distill_topk_bwd_kernel<T, NT, U>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, teacher, ids, k, log2_scale(temperature), \
-                temperature, reinterpret_cast<const float4*>(row_stats), dloss, static_cast<T*>(dlogits), V, parts);                                          \
+                temperature, reinterpret_cast<const float4*>(row_stats), dloss, static_cast<T*>(dlogits), V, parts); \
   } while (0)
-  BY_TYPE(type, BACKWARD, rows, pieces, CALL);
+  BY_TYPE(type, BACKWARD, rows, pieces, 4, CALL);
 #undef CALL
   RTE_LAUNCH_CHECK();
   return RTE_OK;
