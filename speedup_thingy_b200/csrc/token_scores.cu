@@ -942,12 +942,12 @@ void launch_cluster(K kernel, long long ctas, int nt, size_t smem, int C, cudaSt
   (void)cudaLaunchKernelEx(&cfg, kernel, args...);               // (an error stays pending for RTE_LAUNCH_CHECK)
 }
 
-// CTAs per row: as many (up to 8) as come to ten on an SM, with a tile of pieces each; to four where their lists have to be joined too.
-// us, 1 | 2 | 4 | 8 per row: 300 x 50257 bf16 13.1 | 12.4 | 10.3 | 15.6, 700 x 50257 21 | 15.6 | 18.8 | 30; with lists 61 x 131072 fp32
-// 42 | 29 | 20 | 19, 1000 x 32768 bf16 31 | 38 | 55 | 103.
+// CTAs per row: as many (up to 8) as come to ten on an SM, with a tile of pieces each; to four where their lists have to be joined too, two if the rows
+// are not that long.  us, 1 | 2 | 4 | 8 per row: 300 x 50257 bf16 13.1 | 12.4 | 10.3 | 15.6, 700 x 50257 21 | 15.6 | 18.8 | 30; with lists 61 x 131072 fp32
+// 42 | 29 | 20 | 19, 150 x 32768 bf16 11.2 | 13.7, 1000 x 32768 31 | 38 | 55 | 103.
 int cluster_of(long long rows, int pieces, int tile, bool lists) {
   int C = 1;
-  while (C < 8 && rows * C * 2 <= (lists ? 4 : 10) * 148 && pieces > C * tile) C *= 2;
+  while (C < 8 && rows * C * 2 <= (!lists ? 10 : pieces > 8 * tile ? 4 : 2) * 148 && pieces > C * tile) C *= 2;
   return C;
 }
 // The most pieces a row of V columns has: one more where rows do not all start on 16 bytes.
