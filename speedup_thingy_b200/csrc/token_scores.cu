@@ -218,7 +218,7 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
 // other piece holds only what k logits come before.  So the search goes over pieces, an eighth or a quarter of the columns: those that
 // reach a bound are noted, the bound is the k-th of what has been seen (the first one the k-th of the threads' largest, so that a
 // few more than k pieces of a tile pass), and only in the end the columns of the last k pieces, and a few more, are ordered.
-__host__ __device__ constexpr int slack_of(int k) { return k / 2 + 16 + ((k + k / 2) & 1); }       // (k + slack is even)
+__host__ __device__ constexpr int slack_of(int k) { return (k < 64 ? k : 64) + 32 + (k < 64 ? 0 : k & 1); }       // (k + slack is even)
 struct TopK {                                            // in shared memory, sized by k: `shared_bytes`
   struct Head { unsigned long long bound; int count, keep, from, pad[3]; };
   Head& h;
@@ -263,17 +263,16 @@ __device__ __forceinline__ void append(unsigned long long* to, int* count, bool 
   if (mine) to[at + __popc(who & ((1u << (threadIdx.x & 31)) - 1))] = key;
 }
 
-// The largest bound that at least k (at most k + slack, unless equal keys forbid) of n keys reach; one warp, keys STEP words apart.
-// SHIFT: the low bits of a key that say nothing (a 16-bit logit's are all 0 or all 1), not searched.
-template <int SHIFT, int STEP, int HELD>                 // HELD: keys a lane has in registers; more are read again
-__device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int k, int slack, int* reach) {
+// The largest bound that at least k (at most k + slack, unless equal keys forbid) of n keys reach; one warp.  Its lanes hold HELD keys each
+// (0: none, below every bound), more are read from keys[i * STEP], i from 32 * HELD on.  SHIFT: the low bits of a key that say
+// nothing (a 16-bit logit's are all 0 or all 1), not searched.
+template <int SHIFT, int STEP, int HELD>
+__device__ __forceinline__ uint32_t search_bound(const uint32_t (&held)[HELD], const uint32_t* keys, int n, int k, int slack, int* reach) {
   const int lane = threadIdx.x & 31;
-  uint32_t held[HELD], lo = 0xffffffffu, hi = 0;
+  uint32_t lo = 0xffffffffu, hi = 0;
 #pragma unroll
   for (int u = 0; u < HELD; ++u) {
-    const int i = lane + 32 * u;
-    held[u] = i < n ? keys[i * STEP] : 0;                // (0 is below every bound)
-    lo = min(lo, held[u] - 1);                           // (and its predecessor above all)
+    lo = min(lo, held[u] - 1);                           // (the predecessor of 0 is above all)
     hi = max(hi, held[u]);
   }
   for (int i = lane + 32 * HELD; i < n; i += 32) { lo = min(lo, keys[i * STEP] - 1); hi = max(hi, keys[i * STEP]); }
@@ -296,6 +295,16 @@ __device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int 
   }
   *reach = at_lo;
   return lo << SHIFT;
+}
+template <int SHIFT, int STEP, int HELD>
+__device__ __forceinline__ uint32_t warp_bound(const uint32_t* keys, int n, int k, int slack, int* reach) {
+  uint32_t held[HELD];
+#pragma unroll
+  for (int u = 0; u < HELD; ++u) {
+    const int i = (threadIdx.x & 31) + 32 * u;
+    held[u] = i < n ? keys[i * STEP] : 0;
+  }
+  return search_bound<SHIFT, STEP, HELD>(held, keys, n, k, slack, reach);
 }
 
 // A bound that at least k and at most k + slack of n distinct keys reach, n > k + slack; one warp.
@@ -348,15 +357,26 @@ template <int NT, int COUNT, int SHIFT>
 __device__ __forceinline__ void note(TopK& S, float all, int first, int end, bool start) {
   constexpr int round = NT * COUNT;
   const int tid = threadIdx.x;
+  const int have = first < end ? min((end - first + NT - 1) / NT, COUNT) : 0;
   if (start) {
-    const int n = min(end - (first - tid), NT);          // threads with a piece
-    S.top[tid] = value_key(all);
-    if (tid == 0) S.h.count = 0;
-    sync<NT>();
-    if (tid < 32) {
-      int reach;
-      const uint32_t b = n > S.k ? warp_bound<SHIFT, 1, NT / 32>(S.top, n, S.k, S.k / 8, &reach) : 0;
-      if (tid == 0) S.h.bound = (unsigned long long)b << 32;
+    uint32_t b = 0;
+    int reach;
+    if (NT == 32) {                                      // a warp knows all of its pieces
+      const int n = min(end - (first - tid), round);
+      uint32_t key[COUNT];
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j) key[j] = j < have ? value_key(S.tops[j * NT + tid]) : 0;
+      if (n > S.k) b = search_bound<SHIFT, 1, COUNT>(key, nullptr, n, S.k, S.k / 8, &reach);
+      if (tid == 0) { S.h.count = 0; S.h.bound = (unsigned long long)b << 32; }
+    } else {
+      const int n = min(end - (first - tid), NT);        // threads with a piece
+      S.top[tid] = value_key(all);
+      if (tid == 0) S.h.count = 0;
+      __syncthreads();
+      if (tid < 32) {
+        if (n > S.k) b = warp_bound<SHIFT, 1, NT / 32>(S.top, n, S.k, S.k / 8, &reach);
+        if (tid == 0) S.h.bound = (unsigned long long)b << 32;
+      }
     }
     sync<NT>();
   }
@@ -366,7 +386,6 @@ __device__ __forceinline__ void note(TopK& S, float all, int first, int end, boo
 #pragma unroll
   for (int j = 0; j < COUNT; ++j)
     if (!(S.tops[j * NT + tid] < least)) mine |= 1u << j;
-  const int have = first < end ? min((end - first + NT - 1) / NT, COUNT) : 0;
   mine &= (1u << have) - 1;
   int2 at = reserve(&S.h.count, __popc(mine));
   const bool full = at.y > S.cap - round;
@@ -388,7 +407,7 @@ template <int NT, int SHIFT>
 __device__ __forceinline__ void shorten(TopK& S) {
   sync<NT>();
   const int n = S.h.count;
-  if (n > S.k + S.k / 8 + 8) {                             // (they are ordered by counting: n^2 comparisons)
+  if (n > TopK::most(S.k)) {                             // (what is left is ordered by counting, n^2 comparisons)
     thin<NT, SHIFT>(S, S.column_list(), n, S.k / 8 + 8);
     if (threadIdx.x == 0) S.h.from = 0;
   } else if (threadIdx.x == 0) {
@@ -414,24 +433,37 @@ __device__ __forceinline__ void columns(TopK& S, const Row<T>& row) {
   if (threadIdx.x == 0) { S.h.count = 0; S.h.bound = bound; }
   sync<NT>();
   const float least = key_value(bound);
-#pragma unroll 2
-  for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += NT) {
-    float x[N];
-    uint32_t mine = 0;
-    int c = 0;
-    if (i < n) {
-      const int v = (int)~(uint32_t)from[i];
-      Vec<T>::unpack(row.load(v), x);
-      c = row.column(v);
+  for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < n; i0 += 2 * NT) {          // two pieces a thread, both requested at once
+    uint4 raw[2];
+    int c[2];
+    uint32_t mine[2] = {0, 0};
 #pragma unroll
-      for (int j = 0; j < N; ++j) if (!(x[j] < least)) mine |= 1u << j;
-      if (!row.whole(v))
-        for (int j = 0; j < N; ++j) if (c + j < 0 || c + j >= row.V) mine &= ~(1u << j);
+    for (int u = 0; u < 2; ++u) {
+      if (i0 + u * NT >= n) continue;
+      const int v = (int)~(uint32_t)from[i0 + u * NT];
+      raw[u] = row.load(v);
+      c[u] = row.column(v);
     }
-    int2 at = reserve(&S.h.count, __popc(mine));
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (mine >> j & 1) S.column_list()[at.x++] = order_key(x[j], c + j);
+    for (int u = 0; u < 2; ++u) {
+      if (i0 + u * NT >= n) continue;
+      float x[N];
+      Vec<T>::unpack(raw[u], x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) if (!(x[j] < least)) mine[u] |= 1u << j;
+      if (c[u] < 0 || c[u] + N > row.V)
+        for (int j = 0; j < N; ++j) if (c[u] + j < 0 || c[u] + j >= row.V) mine[u] &= ~(1u << j);
+    }
+    int2 at = reserve(&S.h.count, __popc(mine[0]) + __popc(mine[1]));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (mine[u] == 0) continue;
+      float x[N];
+      Vec<T>::unpack(raw[u], x);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (mine[u] >> j & 1) S.column_list()[at.x++] = order_key(x[j], c[u] + j);
+    }
   }
   shorten<NT, Vec<T>::SHIFT>(S);
 }
