@@ -344,7 +344,7 @@ __device__ __forceinline__ void thin(TopK& S, const unsigned long long* keys, in
   }
   sync<NT>();
   const unsigned long long b = S.h.bound;
-  for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += NT) {
+  for (int i = threadIdx.x; (i & ~31) < n; i += NT) {
     const unsigned long long key = i < n ? keys[i] : 0;
     append(S.kept, &S.h.keep, i < n && key >= b, key);
   }
@@ -433,7 +433,7 @@ __device__ __forceinline__ void columns(TopK& S, const Row<T>& row) {
   if (threadIdx.x == 0) { S.h.count = 0; S.h.bound = bound; }
   sync<NT>();
   const float least = key_value(bound);
-  for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < n; i0 += 2 * NT) {          // two pieces a thread, both requested at once
+  for (int i0 = threadIdx.x; (i0 & ~31) < n; i0 += 2 * NT) {                     // two pieces a thread, both requested at once
     uint4 raw[2];
     int c[2];
     uint32_t mine[2] = {0, 0};
