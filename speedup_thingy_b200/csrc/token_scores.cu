@@ -28,7 +28,7 @@ constexpr double LOG2E = 1.44269504088896340736, LN2_D = 0.693147180559945309417
 constexpr float FAR = 1e36f, LOW = -1e30f;     // exponents (in powers of two) and logits beyond these are taken the careful way
 constexpr float MIN_T = 1e-6f, MAX_T = 1e6f;   // temperatures: LOW is then far from all ordinary logits and within fp32 after scaling
 
-__device__ __forceinline__ float exp2_fast(float t) {            // two units in the last place, 0 below -126
+__device__ __forceinline__ float exp2_fast(float t) {            // relative error up to 2^-22.5, 0 below -126
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
@@ -576,7 +576,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   rte::after_previous_grid();
   extern __shared__ __align__(16) unsigned char dyn[];
   TopK top(dyn, k, NT, NT * U * round_tiles(NT, U));                                     // (there is none without TOP)
-  __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
+  __shared__ Sums red[NT / 32];
   __shared__ Sums mine;
   const long long row_at = blockIdx.x / C;
   const int rank = blockIdx.x % C, tid = threadIdx.x;
@@ -675,26 +675,9 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   }
 }
 
-template <int NT>
-__device__ __forceinline__ double block_sum_double(double v, double* red) {
+__device__ __forceinline__ double warp_sum_double(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (NT == 32) return v;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0;
-  for (int w = 0; w < NT / 32; ++w) v += red[w];
-  return v;
-}
-template <int NT>
-__device__ __forceinline__ float block_max_float(float v, float* red) {
-  v = rte::warp_max(v);
-  if (NT == 32) return v;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  for (int w = 0; w < NT / 32; ++w) v = fmaxf(v, red[w]);
   return v;
 }
 
@@ -708,23 +691,20 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   __shared__ __align__(16) int id[TS_MAX_LIST];
   __shared__ float listed[TS_MAX_LIST];                          // the student's logits on the list
   __shared__ uint32_t bits[TAIL ? NT * U * MAP_TILES * Vec<T>::N / 32 : 1];
-  __shared__ Sums red[NT / 32 > 0 ? NT / 32 : 1];
-  __shared__ double red_d[NT / 32 > 0 ? NT / 32 : 1];
-  __shared__ float red_f[NT / 32 > 0 ? NT / 32 : 1];
+  __shared__ Sums red[NT / 32];
   __shared__ Sums mine;
   const long long row_at = blockIdx.x / C;
   const int rank = blockIdx.x % C, tid = threadIdx.x;
   const float* t = teacher + row_at * k;
   const Row<T> row(logits + row_at * ld, V);
   bool any = false;
-  float tmax = -INFINITY;
+  float tmax = -INFINITY;                                        // the list's largest
   for (int i = tid; i < k; i += NT) {
     const long long v = ids[row_at * k + i];
     if (v >= V && status) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
     id[i] = v < 0 || v >= V ? -1 : (int)v;
     if (id[i] < 0) continue;
     any |= TAIL || t[i] != -INFINITY;
-    tmax = fmaxf(tmax, t[i]);
     listed[i] = row.at(id[i]);
   }
   any = __syncthreads_or(any);
@@ -765,18 +745,20 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   } else if (careful(a, c)) {
     a = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
   }
-  // in 64 bits from here: a few values per row, whose small differences are the loss
+  // The rest is one warp's (all of them took turns at it: 13.4 K instructions a row of 32768 with a list of 64), and in 64 bits: a few values
+  // per row, whose small differences are the loss.
+  if (tid >= 32) return;
   const double inv_t = 1. / temp;
   float top = a.top;                                             // the row's largest logit
   const double shift = far(a.top, c) ? 0. : (double)a.top * c - reference(a.top, c);      // log2 of what a.s is too large by
   double s = a.s * exp2(-shift), ln_factor = 0;                  // the row's sum relative to `top`; ln of what a.s is relative to less than it
   if (TAIL) {
-    float m = -INFINITY;
-    for (int i = tid; i < k; i += NT) if (id[i] >= 0) m = fmaxf(m, listed[i]);
-    top = block_max_float<NT>(fmaxf(m, a.top), red_f);
+    float m = a.top;
+    for (int i = tid; i < k; i += 32) if (id[i] >= 0) m = fmaxf(m, listed[i]);
+    top = rte::warp_max(m);
     double l = 0;
     if (top != -INFINITY)
-      for (int i = tid; i < k; i += NT) {
+      for (int i = tid; i < k; i += 32) {
         bool again = id[i] < 0;                                  // a token that an earlier slot names too counts once
         for (int j = 0; j < i; j += 4) {
           const int4 v = *reinterpret_cast<const int4*>(id + j);
@@ -784,7 +766,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
         }
         if (!again) l += expf((float)((listed[i] - (double)top) * inv_t));
       }
-    l = block_sum_double<NT>(l, red_d);
+    l = warp_sum_double(l);
     ln_factor = a.s == 0.f ? 0. : ((double)a.top - top) * inv_t;
     s = l + s * exp(ln_factor);
   }
@@ -792,22 +774,22 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   const bool none = top == -INFINITY && s == 0;                  // nothing but -inf
   double t_shift = 0;
   if (!TAIL) {
-    const float m = block_max_float<NT>(tmax, red_f);
+    float m = -INFINITY;
+    for (int i = tid; i < k; i += 32) if (id[i] >= 0) m = fmaxf(m, t[i]);
+    tmax = rte::warp_max(m);
     double l = 0;
-    for (int i = tid; i < k; i += NT) if (id[i] >= 0) l += exp((double)t[i] - m);
-    l = block_sum_double<NT>(l, red_d);
-    tmax = m;
-    t_shift = log(l);
+    for (int i = tid; i < k; i += 32) if (id[i] >= 0) l += exp((double)t[i] - tmax);
+    t_shift = log(warp_sum_double(l));
   }
   double M = 0, L = 0;
-  for (int i = tid; i < k; i += NT) {
+  for (int i = tid; i < k; i += 32) {
     if (id[i] < 0) continue;
     const double lq = TAIL ? (double)t[i] : (double)t[i] - tmax - t_shift, q = exp(lq);
     M += q;
     if (q != 0) L += q * (lq - (none ? -INFINITY : (listed[i] - (double)top) * inv_t - ln_s));
   }
-  M = block_sum_double<NT>(M, red_d);
-  L = block_sum_double<NT>(L, red_d);
+  M = warp_sum_double(M);
+  L = warp_sum_double(L);
   if (tid != 0) return;
   double P = 1;                                                  // the others' probability
   if (TAIL) {
