@@ -307,14 +307,14 @@ int rte_ce_gradient(const void* logits, int32_t f32, int32_t ldl, const int64_t*
  *   int64 [rows, top_k] in descending order (equal logits: lower column first; NaN above all).  A row whose token is ignore_index (or
  *   out of range, which sets status) is not read: zeros, ids -1.  A row of nothing but -inf: log probabilities -inf, entropy 0.
  *   row_stats f32 [rows, 2] is kept for backward (NULL: none follows; so for distillation).
- * rte_token_logprobs_bwd: dlogits [rows, V] contiguous, of `type`, from the gradients of logprob, entropy and top_logprobs (NULL: none);
+ * rte_token_logprobs_bwd: dlogits [rows, V] contiguous, of `type`, apart from logits, from the gradients of logprob, entropy and top_logprobs (NULL: none);
  *   zeros in rows without a token or a finite logit.
  * rte_distill_topk_fwd: loss f32 [rows] = temperature^2 * KL(teacher || softmax(logits / temperature)).  The teacher's row is a list of
  *   k log probabilities (teacher f32 [rows, k]) at ids int64 [rows, k]; a negative id is an unused slot (one >= V too, and sets status), an
  *   id named twice counts with both.  tail = 0: the list is renormalised, so any constant may be added to a row; tail = 1: what it lacks
  *   of one, max(0, 1 - sum), is the probability of all other tokens together (left out where the student gives them none).  A row
  *   without a used slot or teacher probability (tail = 0) has loss and gradient zero and is not read.  row_stats f32 [rows, 8], on 16 bytes.
- * rte_distill_topk_bwd: dlogits [rows, V] contiguous, of `type`, from dloss f32 [rows].                                            */
+ * rte_distill_topk_bwd: dlogits [rows, V] contiguous, of `type`, apart from logits, from dloss f32 [rows].                                           */
 enum { RTE_TYPE_BF16 = 0, RTE_TYPE_F32 = 1, RTE_TYPE_F16 = 2 };
 enum { RTE_TOKEN_LIST_MAX = 256 };
 int rte_token_logprobs_fwd(const void* logits, int32_t type, int64_t ldl, const int64_t* tokens, int64_t ignore_index, float temperature,

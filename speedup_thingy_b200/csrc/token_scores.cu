@@ -659,12 +659,14 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   const unsigned long long* list = TOP && top.h.from ? top.column_list() : top.kept;
   if (tid >= max(n, 1)) return;
   // ln of the sum relative to the largest logit: without the rounding of R
-  const float ln_s = logf(a.s) - LN2 * (far(a.top, c) ? 0.f : fmaf(a.top, c, -a.R));
+  float ln_s = logf(a.s) - LN2 * (far(a.top, c) ? 0.f : fmaf(a.top, c, -a.R));
+  if (ln_s < 0.f) ln_s = 0.f;                                    // (the largest logit alone makes it 0; no log probability above 0)
   const auto log_p = [&](float x) { return none ? -INFINITY : (x - a.top) * inv_t - ln_s; };
   if (tid == 0) {
     logprob[row_at] = log_p(target);
     // H = ln s - sum t 2^t / s, relative to the same R
-    entropy[row_at] = none ? 0.f : LN2 * (log2f(a.s) - a.e / a.s);
+    const float H = LN2 * (log2f(a.s) - a.e / a.s);
+    entropy[row_at] = none || H < 0.f ? 0.f : H;
     if (stats) stats[row_at] = make_float2(a.top, none ? -INFINITY : log2f(a.s));
   }
   for (int i = tid; i < n; i += NT) {                            // the list's order: how many keys come before

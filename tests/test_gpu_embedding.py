@@ -104,6 +104,21 @@ def test_table_and_rows_beyond_32_bits():
     assert (dw[-1] == 4.0).all() and (dw[-2] == 2.0).all() and (dw[0] == 2.0).all() and not dw[1:-2].any()
 
 
+@pytest.mark.parametrize("n", [100, 9000])
+def test_ids_of_31_bits(n):
+    V = (1 << 30) + 5
+    w = torch.zeros(V, 1, dtype=torch.bfloat16, device=DEV)
+    ids = torch.randint(0, V, (n,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(n))
+    ids[:4] = torch.tensor([V - 1, 0, V - 1, 1 << 30], device=DEV)
+    w[ids] = 2.0
+    leaf = w.requires_grad_()
+    y = K.k_embedding(ids, leaf, scale=0.5)
+    assert (y == 1).all()
+    dw, = torch.autograd.grad([y], [leaf], [torch.ones_like(y)])
+    assert dw[V - 1].item() == 1.0 and dw[0].item() == 0.5 and dw[1 << 30].item() == 0.5
+    assert (dw[ids] >= 0.5).all() and dw.count_nonzero().item() == ids.unique().numel()
+
+
 def test_ids_outside_the_table_are_noted():
     w = torch.randn(20, 16, device=DEV)
     ops = K._ops_for(w)

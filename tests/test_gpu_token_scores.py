@@ -96,6 +96,8 @@ def check_scores(x, tokens, k, T, backward=True, seed=0):
     dx, = torch.autograd.grad([out.logprob, out.entropy, out.top_logprobs], [leaf], [g, gh, gt])
     assert dx.shape == x.shape and dx.dtype == dtype
     want = scores_gradient64(r, g, gh, gt)
+    # (a gradient beyond the type's largest value rounds to infinity: 64 / T at the lowest temperatures in fp16, whose largest is 65504)
+    want = torch.where(want.to(dtype).isinf(), want.to(dtype).double(), want)
     # p is off by err and by the roundings of its argument; what it multiplies by a few half steps of its terms
     every = g.abs() + gt.abs().sum(-1)
     inner = (every[..., None] + gh.abs()[..., None] * (2 * lnv + r["logp"].abs().nan_to_num(0, 0, 0))).double()
@@ -159,6 +161,27 @@ def test_masked_logits(V, dtype):
             assert out.top_ids[1].tolist() == list(range(k)) and (out.top_logprobs[1] == -INF).all()
     assert out.entropy[2] == 0 and out.logprob[2] == 0
     assert abs(out.entropy[4].item() - math.log(V)) < 1e-5 * math.log(V)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1e-6, 1e-3, 50.0, 1e6])
+@pytest.mark.parametrize("V", [50, 3000, 40001])
+def test_temperatures_at_the_ends_of_their_range(V, T, dtype):
+    x = made(4, V, dtype)
+    x[1] *= 0.01
+    x[2] = -3.0                                                  # all equal
+    x[3].masked_fill_(torch.arange(V, device=DEV) % 3 == 0, -INF)
+    tokens = torch.tensor([1, V - 2, 2, 4], device=DEV)
+    out = check_scores(x, tokens, 5, T)
+    assert (out.logprob <= 0).all() and (out.entropy >= 0).all() and (out.top_logprobs <= 0).all()
+
+
+def test_entropies_and_log_probabilities_keep_their_sign():
+    x = torch.zeros(4000, 37, device=DEV)
+    x[:, 5] = torch.linspace(0, 60, 4000, device=DEV)            # up to a certain token
+    for row_type in TYPES:
+        out = K.k_token_logprobs(x.to(row_type), torch.full((4000,), 5, device=DEV), top_k=3, temperature=0.37)
+        assert (out.logprob <= 0).all() and (out.entropy >= 0).all() and (out.top_logprobs <= 0).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -406,6 +429,29 @@ def test_a_listed_id_outside_the_vocabulary_is_noted():
         ops.check_status()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V, T", [(50, 0.02), (3000, 60.0), (40001, 0.1), (3000, 1e3)])
+def test_distillation_at_low_and_high_temperatures(V, T, tail, dtype):
+    x = made(5, V, dtype)
+    check_distill(x, *a_teacher(x, 9, T), T, tail)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_teacher_that_is_not_a_number_stays_in_its_row(tail):
+    x = made(5, 900, torch.float32)
+    t, ids = a_teacher(x, 6, 1.0)
+    want = K.k_distill_topk(x, t, ids, tail=tail)
+    t = t.clone()
+    t[1, 2] = float("nan")
+    t[3] = float("nan")
+    leaf = x.clone().requires_grad_()
+    loss = K.k_distill_topk(leaf, t, ids, tail=tail)
+    dx, = torch.autograd.grad([loss.sum()], [leaf])
+    assert loss[[1, 3]].isnan().all() and torch.equal(loss[[0, 2, 4]], want[[0, 2, 4]])
+    assert dx[[1, 3]].isnan().any(-1).all() and dx[[0, 2, 4]].isfinite().all()
+
+
 def test_distillation_views_and_types_of_the_list():
     x = made(6, 4000, torch.bfloat16).view(2, 3, 4000)
     t, ids = a_teacher(x[..., :1000], 8, 2.0)
@@ -509,6 +555,31 @@ def test_without_a_gradient_the_same_results(rows, V):
         assert torch.equal(K.k_distill_topk(x, t, ids, tail=tail), K.k_distill_topk(leaf, t, ids, tail=tail))
     with torch.no_grad():
         assert not K.k_token_logprobs(leaf, tokens).logprob.requires_grad and not K.k_distill_topk(leaf, t, ids).requires_grad
+
+
+def test_two_threads_on_streams_of_their_own():
+    import threading
+
+    jobs = [(made(40, 9000, torch.bfloat16, seed=i), torch.randint(0, 9000, (40,), device=DEV)) for i in range(2)]
+    want = [_passes(x, tok, *a_teacher(x, 16, 1.2), torch.ones(40, device=DEV)) for x, tok in jobs]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        x, tok = jobs[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = _passes(x, tok, *a_teacher(x, 16, 1.2), torch.ones(40, device=DEV))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(want, got):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
 
 
 def test_logits_changed_in_place_are_refused_by_backward():
