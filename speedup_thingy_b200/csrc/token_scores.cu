@@ -671,7 +671,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   }
   for (int i = tid; i < n; i += NT) {                            // the list's order: how many keys come before
     const unsigned long long key = list[i];
-    int before = 0;
+    int before = 0;                                              // (a bitonic network of one warp instead: 183 us for 159, 35 for 31)
 #pragma unroll 4
     for (int j = 0; j + 1 < n; j += 2) {                         // (the lists start on 16 bytes)
       const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + j);
@@ -906,8 +906,10 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 2048 / NT)
 distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, float temp,
                         const float4* __restrict__ stats, const float* __restrict__ dloss, T* __restrict__ dlogits, int V, int parts) {
   rte::after_previous_grid();
+  constexpr int MAP = NT * U * Vec<T>::N / 32;
   __shared__ int id[TS_MAX_LIST];
   __shared__ float q[TS_MAX_LIST];
+  __shared__ uint32_t map[MAP];                                  // a bit per column of the slice
   const long long row_at = blockIdx.x / parts;
   const int part = blockIdx.x % parts, tid = threadIdx.x;
   const float4 st = stats[row_at * 2];
@@ -926,7 +928,10 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
   const bool is_far = far(list.z, c);
   const Far from(list.z, c);
   const Near near(list.z, c);
+  for (int i = tid; i < MAP; i += 32) map[i] = 0;
+  __syncwarp();
   int n = 0;                                                     // the slots that name a column of this slice, in their order
+  bool twice = false;
   for (int i = tid; i - tid < k; i += 32) {
     const long long j = i < k ? ids[row_at * k + i] : -1;
     const bool mine = slice.holds(j, part);
@@ -935,15 +940,20 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
       const int at = n + __popc(who & ((1u << tid) - 1));
       id[at] = (int)j;
       q[at] = expf(teacher[row_at * k + i] - list.x - list.y);
+      const int bit = (int)j + slice.row.off - part * NT * U * Vec<T>::N;
+      twice |= atomicOr(&map[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1;
     }
     n += __popc(who);
   }
-  __syncwarp();
+  twice = __any_sync(0xffffffffu, twice);
   for (int i = tid; i < n; i += 32) {
     bool again = false;                                          // a token named by several slots: the first of them writes
-    float sum = 0.f;
-    for (int j = 0; j < n; ++j)
-      if (id[j] == id[i]) { again |= j < i; sum += q[j]; }
+    float sum = q[i];
+    if (twice) {
+      sum = 0.f;
+      for (int j = 0; j < n; ++j)
+        if (id[j] == id[i]) { again |= j < i; sum += q[j]; }
+    }
     if (again) continue;
     const float x = slice.row.at(id[i]);
     dlogits[row_at * V + id[i]] = Vec<T>::from_f(exp2_fast((is_far ? from(x) : near(x)) - list.w) * inside - scale * sum);
@@ -986,13 +996,13 @@ int pieces_of(const void* x, int type, long long ld, int V) {
 
 // A row of at most one tile of 32 or 128 threads is one CTA of them; longer ones are walked by 256.
 // Forward, who walks a row.  Many short rows: a warp each (us, 8192 x 2048 bf16, warp | 128 threads: 11.0 | 20, with 32 alternatives 39 | 60;
-// 256 rows of it: 6.2 | 4.8).  Many long ones: 128 threads (8192 x 32768 bf16, warp | 128 | 256 | 512: 119 | 97 | 105 | 151), eight loads each for
+// 16384 x 5000 41 | 57, 16384 x 9001 with 50 181 | 225, 16384 x 16000 108 | 98; 256 x 2048: 6.2 | 4.8).  Many long ones: 128 threads (8192 x 32768 bf16, warp | 128 | 256 | 512: 119 | 97 | 105 | 151), eight loads each for
 // scores, four for distillation, which has more to keep (2000 x 131072 with 64 alternatives, 4 | 8: 133 | 118; 8192 x 32768 distilled 127 | 134).
 // Few long ones, where latency counts: 256 threads, eight loads each (1 x 50257 with 20 alternatives, 128 x 4 | 256 x 4 | 256 x 8: 12.8 | 10.7 | 9.2).
 constexpr int MANY_SHORT = 20 * 148, MANY_LONG = 2 * 148;
 #define FORWARD(T, rows, pieces, LOADS, CALL) \
   do { \
-    if (pieces <= 128 || (pieces <= 512 && rows >= MANY_SHORT)) CALL(T, 32, 4); \
+    if (pieces <= 128 || (pieces <= 1280 && rows >= MANY_SHORT)) CALL(T, 32, 4); \
     else if (pieces <= 512) CALL(T, 128, 4); \
     else if (rows >= MANY_LONG) CALL(T, 128, LOADS); \
     else CALL(T, 256, 8); \

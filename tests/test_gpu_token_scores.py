@@ -121,6 +121,27 @@ def test_scores_and_their_gradient(rows, V, k, T, dtype):
     check_scores(x, tokens, k, T)
 
 
+# rows by who walks them: a warp, several tiles of a warp, 128 threads, several tiles of 128, clusters of 2 to 8 CTAs
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, V, k", [(3000, 300, 20), (3000, 2100, 7), (3000, 4601, 40), (2960, 5003, 256), (2961, 9003, 12), (400, 4099, 100), (300, 20011, 30), (740, 9001, 0),
+                                        (370, 17000, 0), (150, 33000, 9), (70, 70001, 50), (30, 65537, 256)])
+def test_every_way_to_walk_a_row(rows, V, k, dtype):
+    x = made(rows, V, dtype)
+    n = torch.arange(V, device=DEV, dtype=torch.float32)
+    x[0], x[1], x[2], x[3] = n / V * 9 - 4, 3 - n / V * 9, 1.25, torch.where(n % 7 == 3, 5.0, -INF)
+    x[4], x[5], x[6] = -INF, torch.finfo(dtype).min, (n / 50).floor() % 23
+    x[7] = torch.where(n == V - 1, 1.0, -INF)
+    tokens = torch.randint(0, V, (rows,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(rows))
+    tokens[9], tokens[3] = -100, 3
+    check_scores(x, tokens, k, 1.0)
+    t, ids = a_teacher(x, 20, 1.0)
+    ids = ids.clone()
+    ids[10], ids[11, 4:] = -1, -1
+    ids[12, 5] = ids[12, 6]
+    for tail in (False, True):
+        check_distill(x[8:], t[8:], ids[8:], 1.0, tail)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [40, 1000, 9001, 70000])
 @pytest.mark.parametrize("order", ["equal", "two values", "ascending", "descending", "zeros of both signs", "one huge", "steps"])
