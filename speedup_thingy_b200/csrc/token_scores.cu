@@ -15,7 +15,7 @@
 // the row from its kept maximum and sum.  Both are bound by HBM as far as they are simple: gradients of 8192 x 32768 bf16 171 us
 // = 6290 GB/s, sums and entropy alone 91 us = 5900 GB/s (8.8 K instructions a row at 67 % of the issue slots are close behind; the
 // special-function unit could do no more than 1.37 times HBM's rate of bf16 logits).  Lists and the rest of a distillation are bound by their
-// instructions: 64 alternatives make it 159 us, a list of 64 left out of the sum 123.
+// instructions: 64 alternatives make it 157 us, a list of 64 left out of the sum 123.
 
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -576,7 +576,7 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
 
 // ---------------------------------------------------------------- forward
 // A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.  us (k = 0 | listed): 8192 x 32768 bf16
-// 91 | 159 (64), 8192 x 2048 11.0 | 31 (32), 61 x 131072 fp32 12 | 19 (8), 1 x 50257 bf16 4.1 | 9.0 (20), 1531 x 50257 31.
+// 91 | 157 (64), 8192 x 2048 11.0 | 31 (32), 61 x 131072 fp32 12 | 19 (8), 1 x 50257 bf16 4.1 | 9.0 (20), 1531 x 50257 31.
 template <typename T, int NT, int U, bool TOP>
 __global__ void __launch_bounds__(NT, min_ctas(NT, U))
 token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens, long long ignore, float c, float inv_t, int k, float* __restrict__ logprob,
@@ -822,8 +822,8 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
 
 // ---------------------------------------------------------------- backward
 // A CTA per NT * U pieces of a row: what all columns get first, from the row's saved maximum and sum; then its first warp writes the
-// listed columns again.  32 registers, so that an SM holds 2048 threads: with 48, scores 181 us and distillation 208 instead of 171 and 172 (8192 x
-// 32768 bf16, 6290 and 6250 GB/s); 1531 x 50257, whose rows start anywhere, 48 us = 6360 GB/s.
+// listed columns again.  32 registers, so that an SM holds 2048 threads: with 48, scores 181 us and distillation 208 instead of 171 and 168 (8192 x
+// 32768 bf16, 6290 and 6400 GB/s); 1531 x 50257, whose rows start anywhere, 48 us = 6360 GB/s.
 template <typename T, int NT, int U>
 struct Slice {
   Row<T> row;

@@ -10,6 +10,9 @@ Every operator is an autograd function whose forward and backward are C-ABI laun
 (csrc/host_ops.cpp, where a launch costs the host 3-4 us and a call 6 more, against 15-20 us per launch from Python); tensors go in and come out as the
 reference's do (fresh outputs, inputs untouched, non-contiguous inputs accepted).
 
+``k_token_logprobs``, ``k_distill_topk`` and ``k_embedding`` have no counterpart in the reference; they stand beside its cross entropy,
+shortlist logits and embedding module (models.py:136) in the table's manner.
+
 There is no fallback: CPU tensors raise ``RuntimeError`` mentioning ``strict_cuda`` whatever the flag says
 (optimized.py:51-55), and a missing library or device raises when the first operator is called.
 GEMM-bearing operators compute in bf16 with fp32 accumulation (the reference's autocast arithmetic) and return
