@@ -175,8 +175,8 @@ int rte_embed_bwd_grouped(const float* dx, float* dtable, int64_t* accum, int32_
                           rte_stream_t stream);
 
 /* The operator table's lookup: out[i, :] = scale * table[ids[i], :], table [V, d] and out [n, d] of `type` (RTE_TYPE_*), both contiguous;
- * an id out of range gives zeros and sets status.  Its gradient: dtable[v, :] = scale * the sum of dy[i, :] over ids[i] == v, in the
- * order of i (fp32, rounded once; reproducible bit for bit), zeros in rows that no id names and in row padding_idx (< 0: none).
+ * an id out of range gives zeros and sets status.  Its gradient: dtable[v, :] = scale * the sum of dy[i, :] over ids[i] == v, in an
+ * order that the ids alone fix (fp32, rounded once; reproducible bit for bit), zeros in rows that no id names and in row padding_idx (< 0: none).
  * scratch: rte_embedding_bwd_scratch(n, d) bytes on 16, any contents.  n <= RTE_EMBEDDING_MAX_TOKENS.                  */
 enum { RTE_EMBEDDING_MAX_TOKENS = 1 << 27 };
 int rte_embedding_fwd(const int64_t* ids, int64_t n, const void* table, int32_t type, int32_t V, int32_t d, float scale, void* out,

@@ -589,7 +589,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   const long long row_at = blockIdx.x / C;
   const int rank = blockIdx.x % C, tid = threadIdx.x;
   const long long tok = tokens[row_at];
-  if (tok < 0 || tok >= V) {
+  if (tok < 0 || tok >= V || tok == ignore) {
     if (rank == 0) {
       if (tok != ignore && status && tid == 0) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
       if (tid == 0) {
@@ -873,7 +873,7 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const int6
   const int part = blockIdx.x % parts, tid = threadIdx.x;
   const float2 st = stats[row_at];
   const Slice<T, NT, U> slice(logits + row_at * ld, dlogits + row_at * V, V, part);
-  if (tok < 0 || tok >= V || st.y == -INFINITY) return slice.zero();
+  if (tok < 0 || tok >= V || st.y == -INFINITY) return slice.zero();          // (an ignored row's sum was kept as 0 too)
   const float g = g_lp ? g_lp[row_at] : 0.f, gh = g_h ? g_h[row_at] : 0.f;
   float all = 0.f;
   for (int i = tid & 31; g_top && i < k; i += 32) all += g_top[row_at * k + i];        // (every warp for itself)

@@ -224,16 +224,14 @@ def k_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0, i
     (at most 256) most likely tokens, in one pass over the logits; statistics and results in fp32, logits bf16, fp16 or fp32.
 
     Alternatives come in descending order of the logits, equal ones by the lower id.  Log probabilities (of the tokens and of the
-    alternatives) and entropies are differentiable.  Where a token is `ignore_index` the row is not read: zeros, ids -1, no gradient.  A
-    token outside the vocabulary is treated so too and noted in the status word (`CudaOps.check_status`).  Logits of -inf have
+    alternatives) and entropies are differentiable.  Where a token is `ignore_index` (any number, a token of the vocabulary too) the row
+    is not read: zeros, ids -1, no gradient.  A token outside the vocabulary is treated so too and noted in the status word (`CudaOps.check_status`).  Logits of -inf have
     probability zero; a row of nothing else has log probabilities -inf, entropy 0 and no gradient.  Backward reads the logits again."""
     _check_scores("k_token_logprobs", logits, temperature, tokens)
     if tokens.dtype not in _ID_TYPES or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"k_token_logprobs: logits [..., V] with integer tokens [...], got {tuple(logits.shape)} with {tokens.dtype} {tuple(tokens.shape)}")
     if not 0 <= top_k <= min(A.TOKEN_LIST_MAX, logits.shape[-1]):
         raise ValueError(f"k_token_logprobs: top_k must be in 0..{min(A.TOKEN_LIST_MAX, logits.shape[-1])}, got {top_k}")
-    if 0 <= ignore_index < logits.shape[-1]:
-        raise ValueError(f"k_token_logprobs: ignore_index {ignore_index} is a token of the vocabulary")
     _require_cuda_tensor(logits, tokens)
     return TokenLogprobs(*_native(logits).token_logprobs(logits, tokens, int(top_k), float(temperature), int(ignore_index)))
 
@@ -242,10 +240,12 @@ def k_distill_topk(logits, teacher_logprobs, teacher_ids, temperature: float = 1
     """Per-row loss temperature^2 * KL(teacher || softmax(logits [..., V] / temperature)) against a teacher of whom only a list is
     kept: log probabilities [..., k] (k at most 256) at `teacher_ids` [..., k], both as `k_token_logprobs` with the same temperature
     gives them.  `tail=False` renormalises the list (any constant may be added to a row, so the teacher's logits / temperature do as
-    well); `tail=True` keeps its probabilities and gives what they lack of one to all other tokens together.
+    well); `tail=True` keeps its probabilities and gives what they lack of one to all other tokens together (nothing, if they sum to one
+    or more, or if the student gives no other token any probability).
 
     Negative ids are unused slots (lists of uneven length), an id named twice counts with both of its entries, one outside the
-    vocabulary is unused too and noted in the status word.  A row without a used slot has loss and gradient zero and is not read.
+    vocabulary is unused too and noted in the status word.  A row without a used slot (renormalised: without any probability) has loss
+    and gradient zero and is not read.
     Only the logits get a gradient; backward reads them again."""
     _check_scores("k_distill_topk", logits, temperature, teacher_logprobs, teacher_ids)
     if teacher_ids.dtype not in _ID_TYPES or not teacher_logprobs.is_floating_point():
@@ -262,8 +262,8 @@ def k_distill_topk(logits, teacher_logprobs, teacher_ids, temperature: float = 1
 # --------------------------------------------------------------------------- embedding
 def k_embedding(ids, weight, scale: float = 1.0, padding_idx: int | None = None):
     """scale * weight[ids] over a table [V, d] in bf16, fp16 or fp32, rounded once; an id outside the table gives zeros and is noted in
-    the status word.  The table's gradient is dense: every row's sum in fp32 in the order of the tokens, so that it is the same bits
-    every time, rounded once; row `padding_idx` gets none."""
+    the status word.  The table's gradient is dense: every row's sum in fp32 in an order that the ids alone fix, so that it is the
+    same bits every time, rounded once; row `padding_idx` gets none."""
     if weight.dtype not in _LOGIT_TYPES or weight.ndim != 2 or 0 in weight.shape or max(weight.shape) >= 2 ** 31 - 1:
         raise ValueError(f"k_embedding: a table [V, d] in bf16, fp16 or fp32, got {weight.dtype} {tuple(weight.shape)}")
     if ids.dtype not in _ID_TYPES or ids.numel() > A.EMBEDDING_MAX_TOKENS:

@@ -240,6 +240,13 @@ def test_ignored_rows_are_not_read(V):
     nan[[0, 1, 3, 4, 6]] = 1.0
     dx, = torch.autograd.grad([out.logprob, out.entropy], [leaf], [nan, nan])      # what comes back for an ignored row is not looked at
     assert (dx[[2, 5, 7]] == 0).all() and dx.isfinite().all()
+    inside = K.k_token_logprobs(leaf, tokens.masked_fill(tokens < 0, 7), ignore_index=7, top_k=6)      # a token of the vocabulary marks padding
+    skipped = (tokens < 0) | (tokens == 7)
+    for a, b in zip(inside, out):
+        assert torch.equal(a[~skipped], b[~skipped])
+    assert not inside.logprob[skipped].any() and (inside.top_ids[skipped] == -1).all()
+    dx, = torch.autograd.grad([inside.logprob, inside.entropy], [leaf], [nan, nan])
+    assert (dx[skipped] == 0).all() and dx.isfinite().all()
     everything = K.k_token_logprobs(x, torch.full_like(tokens, -1), ignore_index=-1, top_k=3)
     assert not everything.logprob.any() and not everything.entropy.any() and (everything.top_ids == -1).all()
 

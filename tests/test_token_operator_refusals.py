@@ -28,7 +28,6 @@ W = torch.zeros(16, 8)
     (lambda: K.k_token_logprobs(X, TOK, temperature=-1.0), "temperature"),
     (lambda: K.k_token_logprobs(X, TOK, temperature=float("nan")), "temperature"),
     (lambda: K.k_token_logprobs(X, TOK, temperature=float("inf")), "temperature"),
-    (lambda: K.k_token_logprobs(X, TOK, ignore_index=0), "is a token of the vocabulary"),
     (lambda: K.k_token_logprobs(X, TOK.to("meta")), "must be on cpu"),
     (lambda: K.k_distill_topk(X.double(), *LIST), "bf16, fp16 or fp32"),
     (lambda: K.k_distill_topk(X, LIST[0], LIST[1].float()), "integer ids"),
