@@ -692,7 +692,7 @@ __device__ __forceinline__ double warp_sum_double(double v) {
 }
 
 // As above; the teacher's list and the student's logits on it are requested ahead of the row.  us: 8192 x 32768 bf16, 64 and the rest 123 (4360
-// GB/s; the listed columns' bits are a third of its instructions), 1999 x 50257 fp16, 50, renormalised, 30 % of the rows empty 34, 256 x 2048 fp32 5.1.
+// GB/s; the listed columns' bits are a quarter of its instructions), 1999 x 50257 fp16, 50, renormalised, 30 % of the rows empty 34, 256 x 2048 fp32 5.1.
 // stats of a row, eight floats: for the columns outside the list (all, without TAIL) their largest logit, log2 of their sum and what
 // their share of it is multiplied by; M (0: no gradient); the list's max, ln of its sum; the row's largest logit, log2 of its sum
 template <typename T, int NT, int U, bool TAIL>
@@ -757,8 +757,8 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   } else if (careful(a, c)) {
     a = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
   }
-  // The rest is one warp's (all of them took turns at it: 13.4 K instructions a row of 32768 with a list of 64), and in 64 bits: a few values
-  // per row, whose small differences are the loss.
+  // The rest is one warp's (with all of them at it 13.4 K instructions a row of 32768 with a list of 64, now 12.2 K), and in 64 bits: a few
+  // values per row, whose small differences are the loss.
   if (tid >= 32) return;
   const double inv_t = 1. / temp;
   float top = a.top;                                             // the row's largest logit
