@@ -21,7 +21,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int SORT_ONE = 8192, ONE_CTAS = 8, ONE_BITS = 8;           // tokens that one cluster sorts, its CTAs, the bits of its digits
+constexpr int SORT_ONE = 49152, ONE_CTAS = 8, ONE_BITS = 8;          // tokens that one cluster sorts, its CTAs, the bits of its digits
 constexpr int SORT_THREADS = 256, SORT_CTAS = 296;                   // of a sort's launch; CTAs at most
 constexpr int SORT_BITS = 10;                                        // of a digit, at most
 constexpr int ROWS_AHEAD = 8, MAX_RANGE = 64;                        // rows a thread has in flight; sorted rows of a range at most
@@ -113,7 +113,7 @@ struct EoScratch {
   float* part;                  // [ranges][2][d]: what a range adds for an id that began before it | that goes on behind it
 };
 // Tokens that a thread of a sort CTA places at a time: few while the CTAs are few (all of them read all of their counts).
-int sort_each(long long n) { return n <= 32768 ? 2 : n <= 65536 ? 4 : 8; }
+int sort_each(long long n) { return n <= 65536 ? 4 : 8; }
 int sort_span(long long n) {                                          // tokens of a sort CTA
   const int tile = SORT_THREADS * sort_each(n);
   return (int)rte::ceil_div64(rte::ceil_div64(n, tile), SORT_CTAS) * tile;
@@ -185,8 +185,9 @@ __device__ __forceinline__ int sums_before(int v, int* warp_total) {
   return at;
 }
 
-// Up to SORT_ONE tokens by the first cluster, a run of neighbouring tokens per CTA; the other clusters fill.  One CTA of 1024 threads took
-// 21 us for 8192 tokens, most of it the rounds of votes on one SM.
+// Up to SORT_ONE tokens by the first cluster, a run of neighbouring tokens per CTA, up to 24 of them a thread; the other clusters fill.  One
+// CTA of 1024 threads took 21 us for 8192 tokens, most of it the rounds of votes on one SM.  Whole gradients, us, launches per digit | one
+// cluster: 16384 x 1024 bf16 of 32768 45 | 37.6, 30000 x 1024 67 | 55, 30000 x 256 of 2000 49 | 38, 45000 x 1024 of 131072 104 | 96.
 __global__ void __cluster_dims__(ONE_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
 embedding_sort_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int passes, int bits, Fill f, int* status) {
   rte::after_previous_grid();
@@ -563,7 +564,7 @@ void launch_sort(const int64_t* ids, int n, int V, long long padding, const EoSc
   for (int p = 0; p < dg.passes; ++p) {
     const bool to_first = (dg.passes - 1 - p) % 2 == 0;
     int *id_out = to_first ? s.id : s.id2, *tok_out = to_first ? s.tok : s.tok2;
-    const auto place = sort_each(n) == 2 ? embedding_place_kernel<2> : sort_each(n) == 4 ? embedding_place_kernel<4> : embedding_place_kernel<8>;
+    const auto place = sort_each(n) == 4 ? embedding_place_kernel<4> : embedding_place_kernel<8>;
     rte::launch(place, ctas + fills, SORT_THREADS, 0, st, ids, id, tok, id_out, tok_out, s.hist, n, V, padding, p, dg.passes, dg.bits, span, ctas,
                 slice(1 + 2 * p, 3 + 2 * p));
     id = id_out;
@@ -619,7 +620,9 @@ extern "C" int rte_embedding_bwd(const int64_t* ids, int64_t n, const void* dy, 
   if (type == RTE_TYPE_F32 && bytes < 4) return RTE_ERR_ALIGNMENT;
   EoScratch s;
   eo_layout(static_cast<char*>(scratch), n, d, &s);
-  // Rows that no token names: with fewer tokens than rows the whole table is filled beside the sort, and the named rows are written again.
+  // Rows that no token names: with no more tokens than rows the whole table is filled beside the sort, and the named rows are written again; else
+  // they are looked for beside the sums (us, filled ahead | looked for: 33333 x 770 fp32 of 50257 69 | 89, 60000 x 2048 bf16 of 131072 188 | 186, 131072 x
+  // 2048 of 131072 241 | 244).
   const bool fill_ahead = n <= V;
   launch_sort(ids, (int)n, V, padding_idx, s, fill_ahead ? static_cast<char*>(dtable) : nullptr, (long long)V * d * (type == RTE_TYPE_F32 ? 4 : 2), status, ST(stream));
 #define CALL(T, B) launch_sum<T, B>(dy, s, (int)n, V, d, scale, dtable, fill_ahead, ST(stream))

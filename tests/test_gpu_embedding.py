@@ -77,7 +77,7 @@ def test_patterns_of_ids(kind, n, V):
 
 
 def test_long_batches_and_heavy_ids():
-    for n, V, d, kind in ((2200000, 50, 2, "same"), (8192, 100, 16, "zipf"), (8193, 100, 16, "zipf"), (8193, 5000, 16, "same"), (8192, 20000, 16, "same"), (700001, 40000, 4, "zipf"), (700001, 3000000, 4, "random"),
+    for n, V, d, kind in ((2200000, 50, 2, "same"), (8192, 100, 16, "zipf"), (8193, 100, 16, "zipf"), (8193, 5000, 16, "same"), (8192, 20000, 16, "same"), (49152, 3000, 8, "zipf"), (49153, 3000, 8, "zipf"), (49152, 70000, 8, "random"), (60000, 70000, 8, "descending"), (48001, 2, 8, "ends"), (700001, 40000, 4, "zipf"), (700001, 3000000, 4, "random"),
                           (640000, 1 << 21, 2, "descending"), (131072, 131072, 72, "zipf"), (100003, 50257, 24, "zipf"), (70000, 9, 136, "random"), (66000, 300, 8, "same"), (300000, 1000, 4, "zipf")):
         check(some_ids(kind, n, V), torch.randn(V, d, device=DEV).bfloat16(), 3.0)
 
