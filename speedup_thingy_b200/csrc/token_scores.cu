@@ -32,8 +32,9 @@ __host__ __device__ constexpr int min_ctas(int nt, int u) { return nt == 32 ? 24
 constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
 constexpr float LN2 = 0.693147180559945309f;
 constexpr double LOG2E = 1.44269504088896340736, LN2_D = 0.693147180559945309417;
-constexpr float FAR = 1e36f, LOW = -1e30f;     // exponents (in powers of two) and logits beyond these are taken the careful way
-constexpr float MIN_T = 1e-6f, MAX_T = 1e6f;   // temperatures: LOW is then far from all ordinary logits and within fp32 after scaling
+constexpr float FAR = 0x1p27f;                 // exponents (in powers of two) beyond this are taken the careful way
+constexpr float LOW = -1e30f;                  // the least logit that enters an entropy's products: far beyond FAR at any temperature
+constexpr float MIN_T = 1e-6f, MAX_T = 1e6f;   // temperatures: LOW is then within fp32 after scaling
 
 __device__ __forceinline__ float exp2_fast(float t) {            // relative error up to 2^-22.5, 0 below -126
   float r;
@@ -161,12 +162,15 @@ struct Row {
 
 // ---------------------------------------------------------------- sums of exponentials
 // Exponents are kept in powers of two relative to R = top * c, top the largest logit, c = log2(e) / T: t = x c - R in one fused step,
-// whose rounded R shifts every t of a row alike and is taken out again at the end.  Logits below LOW count as LOW (what is masked with
-// -inf or the type's lowest value: 2^t is 0, and t is finite, so that t 2^t is 0 too).  A row whose largest logit is itself
-// down there, or whose R is beyond FAR, is summed again, t = (x - top) c; a row of nothing but -inf has the sum 0.
+// whose rounded R shifts every t of a row alike, by up to half a step of R, and is taken out again at the end.  Below |R| = FAR that is 4 at
+// most; from 2^31 on it could be 128, where 2^t is infinite or 0.  So a row whose R is beyond FAR is summed again with t = (x - top) c, and
+// a tile whose largest logit lies below -2 FAR is left out (`masked`): with ordinary logits in the row it counts nothing (FAR
+// powers of two less), without any the row is summed again, and no running R that anything was summed with is lower.  Logits below LOW count
+// as LOW where t is multiplied (t is then finite, so that t 2^t is 0 as 2^t is); a row of nothing but -inf has the sum 0.
 struct Sums { float top, R, s, e; };           // largest logit, reference, sum of 2^t, sum of t 2^t
 __device__ __forceinline__ float reference(float top, float c) { return fmaxf(top, LOW) * c; }
-__device__ __forceinline__ bool far(float top, float c) { return top <= 0.1f * LOW || !(fabsf(top * c) < FAR); }
+__device__ __forceinline__ bool far(float top, float c) { return !(fabsf(top * c) < FAR); }
+__device__ __forceinline__ bool masked(float top, float c) { return top * c <= -2.f * FAR; }
 __device__ __forceinline__ Sums no_sums(float c) { return {-INFINITY, LOW * c, 0.f, 0.f}; }
 __device__ __forceinline__ void move_to(Sums& a, float R) {      // the same sums relative to R >= a.R
   const float d = a.R - R, f = exp2_fast(d);
@@ -523,7 +527,7 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int begin, int end, fl
 #pragma unroll
     for (int u = 0; u < U; ++u) { top[u] = Vec<T>::max(raw[u]); all = max_nan(all, top[u]); }
     if (all > a.top) a.top = all;
-    if (!(all <= 0.1f * LOW)) {                                  // (else nothing but masked logits, or a row that is summed again)
+    if (!masked(all, c)) {                                       // (NaN is not)
       const float R = fmaxf(a.R, reference(a.top, c));
       if (R > a.R) move_to(a, R);
       const Two cc(c, c), negR(-a.R, -a.R);
