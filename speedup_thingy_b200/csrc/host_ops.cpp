@@ -516,8 +516,10 @@ struct Rows {                                 // [..., V] as rows of one stride:
 // The kernels take the number of rows as an int32.
 void count_fits(int64_t n, const char* what) { TORCH_CHECK_VALUE(n < (int64_t(1) << 31), what, ": ", n, " rows in one call"); }
 Tensor grad_f32(const Tensor& g) { return g.defined() ? g.to(F32).contiguous() : Tensor(); }
-// Where nothing asks for a gradient an operator is its launches alone: no node (3 us of the host's time) and nothing kept for backward.
-bool differentiable(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// Where nothing asks for a derivative an operator is its launches alone: no node (3 us of the host's time) and nothing kept for backward.
+// A tangent of forward mode asks for one (whatever the grad mode): the autograd function refuses it.
+bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+bool differentiable(const Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || has_tangent(t); }
 
 struct TokenLogprobs : Function<TokenLogprobs> {
   struct Out { Tensor tok, logprob, entropy, top_lp, top_ids; };
@@ -606,6 +608,7 @@ struct DistillTopk : Function<DistillTopk> {
   }
 };
 Tensor distill_topk(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature, bool tail) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(teacher), "k_distill_topk: jvp is not implemented for the teacher's log probabilities");
   const Tensor t = teacher.detach().to(F32).contiguous(), id = ids.to(torch::kInt64).contiguous();
   return differentiable(logits) ? DistillTopk::apply(logits, t, id, temperature, tail)[0] : DistillTopk::run(logits, t, id, temperature, tail, nullptr);
 }
