@@ -521,6 +521,20 @@ Tensor grad_f32(const Tensor& g) { return g.defined() ? g.to(F32).contiguous() :
 bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
 bool differentiable(const Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || has_tangent(t); }
 
+// A gradient that cannot be differentiated again: where a graph of it is asked for (create_graph), it has an edge to each tensor that it
+// depends on, which raises when it is walked.
+struct FirstDerivative : Function<FirstDerivative> {
+  static variable_list forward(AutogradContext*, const Tensor& dx, const Tensor&, const Tensor&, const Tensor&, const Tensor&) { return {dx}; }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "rte_b200: trying to differentiate twice an operator that has first derivatives only");
+  }
+};
+Tensor first_derivative(const Tensor& dx, const Tensor& of, const variable_list& g) {
+  if (!at::GradMode::is_enabled()) return dx;
+  const auto grad = [&](size_t i) { return i < g.size() && g[i].defined() ? g[i] : dx; };          // (dx: no edge)
+  return FirstDerivative::apply(dx, of, grad(0), grad(1), grad(2))[0];
+}
+
 struct TokenLogprobs : Function<TokenLogprobs> {
   struct Out { Tensor tok, logprob, entropy, top_lp, top_ids; };
   static Out run(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index, Tensor* stats) {
@@ -563,7 +577,7 @@ struct TokenLogprobs : Function<TokenLogprobs> {
       check(rte_token_logprobs_bwd(ptr(x.t), type_of(x.t), x.ld, saved[1].data_ptr<int64_t>(), ctx->saved_data["temperature"].toDouble(), top_k,
                                    saved[4].data_ptr<int64_t>(), f32(saved[2]), f32(saved[3]), f32(gl), f32(gh), f32(gt), ptr(dx), x.rows, x.V, dev.st),
             "rte_token_logprobs_bwd");
-    return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+    return {first_derivative(dx, saved[0], g), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature, int64_t ignore_index) {
@@ -604,7 +618,7 @@ struct DistillTopk : Function<DistillTopk> {
       check(rte_distill_topk_bwd(ptr(x.t), type_of(x.t), x.ld, f32(saved[1]), saved[2].data_ptr<int64_t>(), saved[2].size(-1),
                                  ctx->saved_data["temperature"].toDouble(), f32(saved[3]), f32(dloss), ptr(dx), x.rows, x.V, dev.st),
             "rte_distill_topk_bwd");
-    return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+    return {first_derivative(dx, saved[0], g), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 Tensor distill_topk(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature, bool tail) {
@@ -644,7 +658,7 @@ struct Embedding : Function<Embedding> {
     check(rte_embedding_bwd(id.data_ptr<int64_t>(), n, ptr(dy), type_of(dy), V, d, ctx->saved_data["scale"].toDouble(), dims[2], ptr(dw), ptr(scratch),
                             scratch.numel(), dev.status, dev.st),
           "rte_embedding_bwd");
-    return {Tensor(), dw, Tensor(), Tensor()};
+    return {Tensor(), first_derivative(dw, dw, g), Tensor(), Tensor()};
   }
 };
 Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) {

@@ -12,7 +12,7 @@ reference's do (fresh outputs, inputs untouched, non-contiguous inputs accepted)
 
 ``k_token_logprobs``, ``k_distill_topk`` and ``k_embedding`` have no counterpart in the reference; they stand beside its cross entropy,
 shortlist logits and embedding module (models.py:136) in the table's manner.  They have first derivatives in reverse mode: a tensor with a
-tangent of forward mode raises.
+tangent of forward mode raises, and so does differentiating one of their gradients (``create_graph``) again.
 
 There is no fallback: CPU tensors raise ``RuntimeError`` mentioning ``strict_cuda`` whatever the flag says
 (optimized.py:51-55), and a missing library or device raises when the first operator is called.

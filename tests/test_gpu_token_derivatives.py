@@ -1,4 +1,4 @@
-"""Derivatives that the operators at the two ends of the vocabulary do not have, on a B200: forward mode is refused
+"""Derivatives that the operators at the two ends of the vocabulary do not have, on a B200: forward mode and second derivatives are refused
 by name, never dropped."""
 import pytest
 import torch
@@ -41,3 +41,16 @@ def test_a_teachers_tangent_is_refused():
     x, _, top, ids = inputs()
     with fwd.dual_level(), pytest.raises(RuntimeError, match="jvp"):
         K.k_distill_topk(x, fwd.make_dual(top, torch.ones_like(top)), ids)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_second_derivatives_are_refused(name):
+    x = inputs()[0].requires_grad_()
+    y = CALLS[name](x)
+    g = torch.ones_like(y).requires_grad_()
+    dx, = torch.autograd.grad([y], [x], [g], create_graph=True)
+    plain, = torch.autograd.grad([CALLS[name](x)], [x], [g])
+    assert torch.equal(dx.detach(), plain) and not plain.requires_grad       # the first derivative is as ever
+    for of in (g,) if name == "embedding" else (x, g):           # (a table's gradient does not depend on the table)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            torch.autograd.grad([(dx * dx).sum() + (x * x).sum() + (g * g).sum()], [of], retain_graph=True)
