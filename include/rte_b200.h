@@ -177,8 +177,9 @@ int rte_embed_bwd_grouped(const float* dx, float* dtable, int64_t* accum, int32_
 /* The operator table's lookup: out[i, :] = scale * table[ids[i], :], table [V, d] and out [n, d] of `type` (RTE_TYPE_*), both contiguous;
  * an id out of range gives zeros and sets status.  Its gradient: dtable[v, :] = scale * the sum of dy[i, :] over ids[i] == v, in an
  * order that the ids alone fix (fp32, rounded once; reproducible bit for bit), zeros in rows that no id names and in row padding_idx (< 0: none).
- * scratch: rte_embedding_bwd_scratch(n, d) bytes on 16, any contents.  n <= RTE_EMBEDDING_MAX_TOKENS.                  */
-enum { RTE_EMBEDDING_MAX_TOKENS = 1 << 27 };
+ * scratch: rte_embedding_bwd_scratch(n, d) bytes on 16, any contents.  n <= RTE_EMBEDDING_MAX_TOKENS,
+ * d <= RTE_EMBEDDING_MAX_COLUMNS.                  */
+enum { RTE_EMBEDDING_MAX_TOKENS = 1 << 27, RTE_EMBEDDING_MAX_COLUMNS = 1 << 30 };
 int rte_embedding_fwd(const int64_t* ids, int64_t n, const void* table, int32_t type, int32_t V, int32_t d, float scale, void* out,
                       int32_t* status, rte_stream_t stream);
 int64_t rte_embedding_bwd_scratch(int64_t n, int32_t d);

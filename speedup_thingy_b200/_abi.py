@@ -18,7 +18,7 @@ ROUTER_DPOOLED_PARTS = 4
 ERR_ALIGNMENT, ERR_UNSUPPORTED = -2, -5
 ADAMW_CHUNK = 4096
 TYPE_BF16, TYPE_F32, TYPE_F16 = 0, 1, 2
-TOKEN_LIST_MAX, EMBEDDING_MAX_TOKENS = 256, 1 << 27
+TOKEN_LIST_MAX, EMBEDDING_MAX_TOKENS, EMBEDDING_MAX_COLUMNS = 256, 1 << 27, 1 << 30
 
 
 class GemmArgs(C.Structure):

@@ -525,9 +525,12 @@ int piece_bytes(const void* a, const void* b, long long row_bytes) {
   return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
+// (in 64 bits: d is at most 2^30, a row's bytes are not; the kernels' columns, a grid's width beyond the last, stay within an int)
+template <typename T, int BYTES> int pieces_of(int d) { return int((long long)d * (int)sizeof(T) / BYTES); }
+
 template <typename T, int BYTES>
 void launch_fwd(const int64_t* ids, long long n, const void* table, int V, int d, float scale, void* out, int* status, cudaStream_t st) {
-  const int pieces = d * (int)sizeof(T) / BYTES, tpr = threads_per_row(pieces);
+  const int pieces = pieces_of<T, BYTES>(d), tpr = threads_per_row(pieces);
   const long long ctas = rte::ceil_div64(n, (long long)(128 / tpr) * TOKENS_AHEAD);
   const int columns = (int)min((long long)rte::ceil_div(pieces, tpr), rte::ceil_div64(148 * 8, ctas));      // few tokens: a CTA per 128 pieces
   rte::launch(embedding_fwd_kernel<T, BYTES>, dim3((unsigned)min(ctas, 148LL * 64), columns), 128, 0, st, ids, n, static_cast<const T*>(table), V, pieces, tpr, scale,
@@ -535,7 +538,7 @@ void launch_fwd(const int64_t* ids, long long n, const void* table, int V, int d
 }
 template <typename T, int BYTES>
 void launch_sum(const void* dy, const EoScratch& s, int n, int V, int d, float scale, void* dtable, bool filled, cudaStream_t st) {
-  const int pieces = d * (int)sizeof(T) / BYTES, tpr = max(threads_per_row(pieces), MIN_TPR), range = range_of(n), ranges = rte::ceil_div(n, range);
+  const int pieces = pieces_of<T, BYTES>(d), tpr = max(threads_per_row(pieces), MIN_TPR), range = range_of(n), ranges = rte::ceil_div(n, range);
   const int range_ctas = rte::ceil_div(ranges, 128 / tpr);
   const dim3 grid(range_ctas + (filled ? 0 : rte::ceil_div(V, ZERO_ROWS)), (unsigned)min(rte::ceil_div(pieces, tpr), 64));
   rte::launch(embedding_sum_kernel<T, BYTES>, grid, 128, 0, st, static_cast<const T*>(dy), s, n, V, pieces, tpr, range, d, scale, static_cast<T*>(dtable), range_ctas);
@@ -596,7 +599,7 @@ void launch_sort(const int64_t* ids, int n, int V, long long padding, const EoSc
 
 extern "C" int rte_embedding_fwd(const int64_t* ids, int64_t n, const void* table, int32_t type, int32_t V, int32_t d, float scale, void* out, int32_t* status,
                                  rte_stream_t stream) {
-  RTE_CHECK_ARG(ids && table && out && type_ok(type) && n > 0 && V > 0 && d > 0);
+  RTE_CHECK_ARG(ids && table && out && type_ok(type) && n > 0 && V > 0 && d > 0 && d <= RTE_EMBEDDING_MAX_COLUMNS);
   const int bytes = piece_bytes(table, out, (long long)d * (type == RTE_TYPE_F32 ? 4 : 2));
   if (type == RTE_TYPE_F32 && bytes < 4) return RTE_ERR_ALIGNMENT;
 #define CALL(T, B) launch_fwd<T, B>(ids, n, table, V, d, scale, out, status, ST(stream))
@@ -607,13 +610,14 @@ extern "C" int rte_embedding_fwd(const int64_t* ids, int64_t n, const void* tabl
 }
 
 extern "C" int64_t rte_embedding_bwd_scratch(int64_t n, int32_t d) {
-  if (n <= 0 || d <= 0 || n > RTE_EMBEDDING_MAX_TOKENS) return 0;
+  if (n <= 0 || d <= 0 || n > RTE_EMBEDDING_MAX_TOKENS || d > RTE_EMBEDDING_MAX_COLUMNS) return 0;
   return (int64_t)eo_layout(nullptr, n, d, nullptr);
 }
 
 extern "C" int rte_embedding_bwd(const int64_t* ids, int64_t n, const void* dy, int32_t type, int32_t V, int32_t d, float scale, int64_t padding_idx, void* dtable,
                                  void* scratch, int64_t scratch_bytes, int32_t* status, rte_stream_t stream) {
-  RTE_CHECK_ARG(ids && dy && dtable && scratch && type_ok(type) && n > 0 && n <= RTE_EMBEDDING_MAX_TOKENS && V > 0 && V < 0x7fffffff && d > 0);
+  RTE_CHECK_ARG(ids && dy && dtable && scratch && type_ok(type) && n > 0 && n <= RTE_EMBEDDING_MAX_TOKENS && V > 0 && V < 0x7fffffff && d > 0 &&
+                d <= RTE_EMBEDDING_MAX_COLUMNS);
   if (scratch_bytes < rte_embedding_bwd_scratch(n, d)) return RTE_ERR_SCRATCH_CAPACITY;
   if (reinterpret_cast<uintptr_t>(scratch) & 15) return RTE_ERR_ALIGNMENT;
   const int bytes = piece_bytes(dy, dtable, (long long)d * (type == RTE_TYPE_F32 ? 4 : 2));

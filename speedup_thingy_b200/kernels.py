@@ -265,8 +265,8 @@ def k_embedding(ids, weight, scale: float = 1.0, padding_idx: int | None = None)
     """scale * weight[ids] over a table [V, d] in bf16, fp16 or fp32, rounded once; an id outside the table gives zeros and is noted in
     the status word.  The table's gradient is dense: every row's sum in fp32 in an order that the ids alone fix, so that it is the
     same bits every time, rounded once; row `padding_idx` gets none."""
-    if weight.dtype not in _LOGIT_TYPES or weight.ndim != 2 or 0 in weight.shape or max(weight.shape) >= 2 ** 31 - 1:
-        raise ValueError(f"k_embedding: a table [V, d] in bf16, fp16 or fp32, got {weight.dtype} {tuple(weight.shape)}")
+    if weight.dtype not in _LOGIT_TYPES or weight.ndim != 2 or 0 in weight.shape or weight.shape[0] >= 2 ** 31 - 1 or weight.shape[1] > A.EMBEDDING_MAX_COLUMNS:
+        raise ValueError(f"k_embedding: a table [V, d <= {A.EMBEDDING_MAX_COLUMNS}] in bf16, fp16 or fp32, got {weight.dtype} {tuple(weight.shape)}")
     if ids.dtype not in _ID_TYPES or ids.numel() > A.EMBEDDING_MAX_TOKENS:
         raise ValueError(f"k_embedding: at most {A.EMBEDDING_MAX_TOKENS} integer ids, got {ids.dtype} {tuple(ids.shape)}")
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
