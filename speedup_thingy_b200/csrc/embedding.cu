@@ -91,7 +91,7 @@ embedding_fwd_kernel(const int64_t* __restrict__ ids, long long n, const T* __re
       for (int u = 0; u < TOKENS_AHEAD; ++u) r[u] = id[u] >= 0 ? w[id[u] * pieces + c] : R{};
 #pragma unroll
       for (int u = 0; u < TOKENS_AHEAD; ++u)
-        if (t + u < n) y[(t + u) * pieces + c] = pack<T, BYTES>(unpack<T, BYTES>(r[u]), scale);
+        if (t + u < n) y[(t + u) * pieces + c] = id[u] >= 0 ? pack<T, BYTES>(unpack<T, BYTES>(r[u]), scale) : R{};       // (no product: 0 times infinity)
     }
   }
 }
