@@ -315,6 +315,7 @@ int rte_ce_gradient(const void* logits, int32_t f32, int32_t ldl, const int64_t*
  *   id named twice counts with both.  tail = 0: the list is renormalised, so any constant may be added to a row; tail = 1: what it lacks
  *   of one, max(0, 1 - sum), is the probability of all other tokens together (left out where the student gives them none).  A row
  *   without a used slot or teacher probability (tail = 0) has loss and gradient zero and is not read.  row_stats f32 [rows, 8], on 16 bytes.
+ *   Above a temperature of 8 sums are in 64 bits: the loss would be off by temperature^2 1e-7.
  * rte_distill_topk_bwd: dlogits [rows, V] contiguous, of `type`, apart from logits, from dloss f32 [rows].                                           */
 enum { RTE_TYPE_BF16 = 0, RTE_TYPE_F32 = 1, RTE_TYPE_F16 = 2 };
 enum { RTE_TOKEN_LIST_MAX = 256 };

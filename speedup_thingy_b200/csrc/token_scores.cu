@@ -20,6 +20,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "rte_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -35,6 +37,11 @@ constexpr double LOG2E = 1.44269504088896340736, LN2_D = 0.693147180559945309417
 constexpr float FAR = 0x1p27f;                 // exponents (in powers of two) beyond this are taken the careful way
 constexpr float LOW = -1e30f;                  // the least logit that enters an entropy's products: far beyond FAR at any temperature
 constexpr float MIN_T = 1e-6f, MAX_T = 1e6f;   // temperatures: LOW is then within fp32 after scaling
+// Distillation above this temperature has its sums and its listed columns' gradients in 64 bits: the loss is T^2 times a divergence that falls
+// as T^-2, so that an error of 1e-7 in a row's logarithm, fp32's, is one of T^2 1e-7 in a loss of order one.  The second pass over the row is bound
+// by the fp64 pipe (8192 x 32768 bf16, 64 listed, us forward | backward at T = 8 and above it: 104 | 170 and 502 | 236, with the rest 125 | 168 and
+// 629 | 229), which is why lower temperatures, where that error is below 1e-5, go without.
+constexpr float HOT_T = 8.f;
 
 __device__ __forceinline__ float exp2_fast(float t) {            // relative error up to 2^-22.5, 0 below -126
   float r;
@@ -578,6 +585,47 @@ __device__ __noinline__ Sums sums_far(const Row<T> row, int begin, int end, floa
   return a;
 }
 
+__device__ __forceinline__ double warp_sum_double(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The sum of exp((x - top) / T) over a row's pieces [begin, end) in 64 bits, top not -inf; OUTSIDE and `bits` as in `stream`.
+template <typename T, int NT, int U, bool OUTSIDE>
+__device__ __noinline__ double sum_hot(const Row<T> row, int begin, int end, float top, double inv_t, const int* id, int ids, uint32_t* bits, double* red) {
+  constexpr int N = Vec<T>::N, SPAN = NT * U * MAP_TILES;
+  const int tid = threadIdx.x;
+  double s = 0;
+  for (int at = begin; at < end; at += SPAN) {
+    if (OUTSIDE) {
+      sync<NT>();
+      for (int i = tid; i < SPAN * N / 32; i += NT) bits[i] = 0;
+      sync<NT>();
+      for (int i = tid; i < ids; i += NT) {
+        const int bit = id[i] + row.off - at * N;
+        if (id[i] >= 0 && bit >= 0 && bit < SPAN * N) atomicOr(&bits[bit >> 5], 1u << (bit & 31));
+      }
+      sync<NT>();
+    }
+    for (int v = at + tid; v < min(at + SPAN, end); v += NT) {
+      const int bit = (v - at) * N;
+      const uint32_t listed = OUTSIDE ? bits[bit / 32] >> (bit % 32) : 0;
+      float x[N];
+      Vec<T>::unpack(row.load(v), x);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (!(listed >> i & 1)) s += exp(((double)x[i] - top) * inv_t);
+    }
+  }
+  s = warp_sum_double(s);
+  if (NT == 32) return s;
+  __syncthreads();
+  if (tid % 32 == 0) red[tid / 32] = s;
+  __syncthreads();
+  return warp_sum_double(tid % 32 < NT / 32 ? red[tid % 32] : 0.);
+}
+
 // ---------------------------------------------------------------- forward
 // A cluster of C CTAs per row, each with a slice of its pieces; rank 0 joins what they found.  us (k = 0 | listed): 8192 x 32768 bf16
 // 91 | 157 (64), 8192 x 2048 11.0 | 31 (32), 61 x 131072 fp32 12 | 19 (8), 1 x 50257 bf16 4.1 | 9.0 (20), 1531 x 50257 31.
@@ -689,18 +737,13 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int64_t*
   }
 }
 
-__device__ __forceinline__ double warp_sum_double(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // As above; the teacher's list and the student's logits on it are requested ahead of the row.  us: 8192 x 32768 bf16, 64 and the rest 123 (4360
 // GB/s; the listed columns' bits are a quarter of its instructions), 1999 x 50257 fp16, 50, renormalised, 30 % of the rows empty 34, 256 x 2048 fp32 5.1.
 // stats of a row, eight floats: for the columns outside the list (all, without TAIL) their largest logit, log2 of their sum and what
-// their share of it is multiplied by; M (0: no gradient); the list's max, ln of its sum; the row's largest logit, log2 of its sum
-template <typename T, int NT, int U, bool TAIL>
-__global__ void __launch_bounds__(NT, min_ctas(NT, U))
+// their share of it is multiplied by; M (0: no gradient); the list's max, ln of its sum; the row's largest logit, log2 of its sum.  HOT: of
+// the last four ln of the row's sum over M in 64 bits (two of them), the row's largest logit, whether the list stays as it is (TAIL).
+template <typename T, int NT, int U, bool TAIL, bool HOT>
+__global__ void __launch_bounds__(NT, HOT ? min_ctas(NT, U) / 2 : min_ctas(NT, U))
 distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, double temp,
                     float* __restrict__ loss, float4* __restrict__ stats, int V, int C, int* status) {
   rte::after_previous_grid();
@@ -709,6 +752,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   __shared__ uint32_t bits[TAIL ? NT * U * MAP_TILES * Vec<T>::N / 32 : 1];
   __shared__ Sums red[NT / 32];
   __shared__ Sums mine;
+  __shared__ double red_hot[HOT ? NT / 32 : 1], mine_hot;
   const long long row_at = blockIdx.x / C;
   const int rank = blockIdx.x % C, tid = threadIdx.x;
   const float* t = teacher + row_at * k;
@@ -734,6 +778,8 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   const int per = (row.pieces + C - 1) / C, begin = min(rank * per, row.pieces), end = min(begin + per, row.pieces);
   Sums a = stream<T, NT, U, false, false, TAIL>(row, begin, end, c, nullptr, id, k, bits);
   a = block_sums<NT>(a, c, red);
+  const double inv_t = 1. / temp;
+  double hot = 0;                                                // HOT: the sum relative to a.top
   if (C > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     if (tid == 0) mine = a;
@@ -747,7 +793,13 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
       a.top = fmaxf(a.top, b.top);
       a.s += b.s;
     }
-    if (careful(a, c)) {
+    if (HOT) {
+      if (a.top != -INFINITY) hot = sum_hot<T, NT, U, TAIL>(row, begin, end, a.top, inv_t, id, k, bits, red_hot);
+      if (tid == 0) mine_hot = hot;
+      cluster.sync();
+      hot = 0;
+      for (int r = 0; r < C; ++r) hot += *cluster.map_shared_rank(&mine_hot, r);
+    } else if (careful(a, c)) {
       const Sums b = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
       cluster.sync();
       if (tid == 0) mine = b;
@@ -758,16 +810,18 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
     }
     cluster.sync();                                              // (the others leave)
     if (rank != 0) return;
+  } else if (HOT) {
+    if (a.top != -INFINITY) hot = sum_hot<T, NT, U, TAIL>(row, begin, end, a.top, inv_t, id, k, bits, red_hot);
   } else if (careful(a, c)) {
     a = sums_far<T, NT, TAIL>(row, begin, end, a.top, c, id, k, red);
   }
   // The rest is one warp's (with all of them at it 13.4 K instructions a row of 32768 with a list of 64, now 12.2 K), and in 64 bits: a few
   // values per row, whose small differences are the loss.
   if (tid >= 32) return;
-  const double inv_t = 1. / temp;
   float top = a.top;                                             // the row's largest logit
+  const bool others = HOT ? hot != 0 : a.s != 0.f;
   const double shift = far(a.top, c) ? 0. : (double)a.top * c - reference(a.top, c);      // log2 of what a.s is too large by
-  double s = a.s * exp2(-shift), ln_factor = 0;                  // the row's sum relative to `top`; ln of what a.s is relative to less than it
+  double s = HOT ? hot : a.s * exp2(-shift), ln_factor = 0;      // the row's sum relative to `top`; ln of what a.s is relative to less than it
   if (TAIL) {
     float m = a.top;
     for (int i = tid; i < k; i += 32) if (id[i] >= 0) m = fmaxf(m, listed[i]);
@@ -780,10 +834,11 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
           const int4 v = *reinterpret_cast<const int4*>(id + j);
           again |= v.x == id[i] || (j + 1 < i && v.y == id[i]) || (j + 2 < i && v.z == id[i]) || (j + 3 < i && v.w == id[i]);
         }
-        if (!again) l += expf((float)((listed[i] - (double)top) * inv_t));
+        const double d = (listed[i] - (double)top) * inv_t;
+        if (!again) l += HOT ? exp(d) : expf((float)d);
       }
     l = warp_sum_double(l);
-    ln_factor = a.s == 0.f ? 0. : ((double)a.top - top) * inv_t;
+    ln_factor = others ? ((double)a.top - top) * inv_t : 0.;
     s = l + s * exp(ln_factor);
   }
   const double ln_s = log(s);
@@ -809,7 +864,7 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   if (tid != 0) return;
   double P = 1;                                                  // the others' probability
   if (TAIL) {
-    const double r = a.s > 0.f ? fmax(0., 1 - M) : 0., ln_out = ln_factor + log((double)a.s) - shift * LN2_D - ln_s;
+    const double r = (HOT ? hot > 0 : a.s > 0.f) ? fmax(0., 1 - M) : 0., ln_out = ln_factor + (HOT ? log(hot) : log((double)a.s) - shift * LN2_D) - ln_s;
     P = exp(ln_out);
     if (r > 0) L += r * (log(r) - ln_out);
     M += r;
@@ -818,9 +873,14 @@ distill_topk_kernel(const T* __restrict__ logits, long long ld, const float* __r
   loss[row_at] = float(L * temp * temp);
   if (!stats) return;
   // 2^-l2 of a sum relative to the rounded reference that backward forms again: the others' among themselves, and the row's
-  const bool others = a.s != 0.f;
+  stats[row_at * 2] = make_float4(others ? a.top : 0.f, others ? HOT ? float(log2(hot) + shift) : log2f(a.s) : 0.f, !others ? 0.f : TAIL ? (float)P : (float)M,
+                                  none ? 0.f : (float)M);
+  if (HOT) {
+    const double A = ln_s - log(M);
+    stats[row_at * 2 + 1] = make_float4(__int_as_float(__double2hiint(A)), __int_as_float(__double2loint(A)), top, TAIL ? 1.f : 0.f);
+    return;
+  }
   const double l2 = ln_s * LOG2E + (far(top, c) ? 0. : (double)top * c - reference(top, c));
-  stats[row_at * 2] = make_float4(others ? a.top : 0.f, others ? log2f(a.s) : 0.f, !others ? 0.f : TAIL ? (float)P : (float)M, none ? 0.f : (float)M);
   stats[row_at * 2 + 1] = make_float4(TAIL ? 0.f : tmax, (float)t_shift, top, (float)l2);
 }
 
@@ -905,14 +965,14 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const int6
   else write(Near(st.x, c));
 }
 
-template <typename T, int NT, int U>
-__global__ void __launch_bounds__(NT, NT == 32 ? 24 : 2048 / NT)
+template <typename T, int NT, int U, bool HOT>
+__global__ void __launch_bounds__(NT, HOT ? 1024 / NT < 16 ? 1024 / NT : 16 : NT == 32 ? 24 : 2048 / NT)
 distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float* __restrict__ teacher, const int64_t* __restrict__ ids, int k, float c, float temp,
                         const float4* __restrict__ stats, const float* __restrict__ dloss, T* __restrict__ dlogits, int V, int parts) {
   rte::after_previous_grid();
   constexpr int MAP = NT * U * Vec<T>::N / 32;
   __shared__ int id[TS_MAX_LIST];
-  __shared__ float q[TS_MAX_LIST];
+  __shared__ std::conditional_t<HOT, double, float> q[TS_MAX_LIST];
   __shared__ uint32_t map[MAP];                                  // a bit per column of the slice
   const long long row_at = blockIdx.x / parts;
   const int part = blockIdx.x % parts, tid = threadIdx.x;
@@ -932,6 +992,18 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
   const bool is_far = far(list.z, c);
   const Far from(list.z, c);
   const Near near(list.z, c);
+  double A = 0, L = 0;                                           // HOT: M p = exp((x - top) / T - A), q = exp(t - L)
+  if (HOT) {
+    A = __hiloint2double(__float_as_int(list.x), __float_as_int(list.y));
+    if (list.w == 0.f) {                                         // the renormalised list's logarithm, as forward formed it
+      float m = -INFINITY;
+      for (int i = tid; i < k; i += 32) { const long long j = ids[row_at * k + i]; if (j >= 0 && j < V) m = fmaxf(m, teacher[row_at * k + i]); }
+      m = rte::warp_max(m);
+      double l = 0;
+      for (int i = tid; i < k; i += 32) { const long long j = ids[row_at * k + i]; if (j >= 0 && j < V) l += exp((double)teacher[row_at * k + i] - m); }
+      L = m + log(warp_sum_double(l));
+    }
+  }
   for (int i = tid; i < MAP; i += 32) map[i] = 0;
   __syncwarp();
   int n = 0;                                                     // the slots that name a column of this slice, in their order
@@ -943,7 +1015,8 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
     if (mine) {
       const int at = n + __popc(who & ((1u << tid) - 1));
       id[at] = (int)j;
-      q[at] = expf(teacher[row_at * k + i] - list.x - list.y);
+      if (HOT) q[at] = exp(teacher[row_at * k + i] - L);
+      else q[at] = expf(teacher[row_at * k + i] - list.x - list.y);
       const int bit = (int)j + slice.row.off - part * NT * U * Vec<T>::N;
       twice |= atomicOr(&map[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1;
     }
@@ -952,15 +1025,16 @@ distill_topk_bwd_kernel(const T* __restrict__ logits, long long ld, const float*
   twice = __any_sync(0xffffffffu, twice);
   for (int i = tid; i < n; i += 32) {
     bool again = false;                                          // a token named by several slots: the first of them writes
-    float sum = q[i];
+    auto sum = q[i];
     if (twice) {
-      sum = 0.f;
+      sum = 0;
       for (int j = 0; j < n; ++j)
         if (id[j] == id[i]) { again |= j < i; sum += q[j]; }
     }
     if (again) continue;
     const float x = slice.row.at(id[i]);
-    dlogits[row_at * V + id[i]] = Vec<T>::from_f(exp2_fast((is_far ? from(x) : near(x)) - list.w) * inside - scale * sum);
+    if (HOT) dlogits[row_at * V + id[i]] = Vec<T>::from_f(float(scale * (exp(((double)x - list.z) / temp - A) - sum)));
+    else dlogits[row_at * V + id[i]] = Vec<T>::from_f(exp2_fast((is_far ? from(x) : near(x)) - list.w) * inside - scale * sum);
   }
 }
 
@@ -1083,11 +1157,13 @@ extern "C" int rte_distill_topk_fwd(const void* logits, int32_t type, int64_t ld
   RTE_CHECK_ARG(rows_ok(logits, type, ldl, rows, V) && teacher && ids && loss && temperature_ok(temperature));
   RTE_CHECK_ARG(k > 0 && k <= TS_MAX_LIST);
   if (!on_element(logits, type) || reinterpret_cast<uintptr_t>(row_stats) % 16) return RTE_ERR_ALIGNMENT;
+  const bool hot = temperature > HOT_T;
   const int pieces = pieces_of(logits, type, ldl, V);
 #define CALL(T, NT, U) \
   do { \
     const int C = cluster_of(rows, pieces, NT * U, false); \
-    launch_cluster(tail ? distill_topk_kernel<T, NT, U, true> : distill_topk_kernel<T, NT, U, false>, (long long)rows * C, NT, 0, C, ST(stream), \
+    launch_cluster(tail ? hot ? distill_topk_kernel<T, NT, U, true, true> : distill_topk_kernel<T, NT, U, true, false> \
+                        : hot ? distill_topk_kernel<T, NT, U, false, true> : distill_topk_kernel<T, NT, U, false, false>, (long long)rows * C, NT, 0, C, ST(stream), \
                    static_cast<const T*>(logits), (long long)ldl, teacher, ids, (int)k, log2_scale(temperature), (double)temperature, loss, \
                    reinterpret_cast<float4*>(row_stats), (int)V, C, status); \
   } while (0)
@@ -1107,7 +1183,7 @@ extern "C" int rte_distill_topk_bwd(const void* logits, int32_t type, int64_t ld
   do { \
     const int parts = rte::ceil_div(pieces, NT * U); \
     if ((long long)rows * parts > 0x7fffffff) return RTE_ERR_UNSUPPORTED; \
-    rte::launch(distill_topk_bwd_kernel<T, NT, U>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, teacher, ids, k, log2_scale(temperature), \
+    rte::launch(temperature > HOT_T ? distill_topk_bwd_kernel<T, NT, U, true> : distill_topk_bwd_kernel<T, NT, U, false>, rows * parts, NT, 0, ST(stream), static_cast<const T*>(logits), ldl, teacher, ids, k, log2_scale(temperature), \
                 temperature, reinterpret_cast<const float4*>(row_stats), dloss, static_cast<T*>(dlogits), V, parts); \
   } while (0)
   BY_TYPE(type, BACKWARD, rows, pieces, 4, CALL);

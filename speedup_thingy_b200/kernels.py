@@ -247,6 +247,8 @@ def k_distill_topk(logits, teacher_logprobs, teacher_ids, temperature: float = 1
     Negative ids are unused slots (lists of uneven length), an id named twice counts with both of its entries, one outside the
     vocabulary is unused too and noted in the status word.  A row without a used slot (renormalised: without any probability) has loss
     and gradient zero and is not read.
+    The loss is off by about temperature^2 10^-7 up to a temperature of 8; above it sums and differences are in 64 bits, so that the loss keeps
+    its digits as the divergence falls (four to five times the time forward where rows are many).
     Only the logits get a gradient; backward reads them again."""
     _check_scores("k_distill_topk", logits, temperature, teacher_logprobs, teacher_ids)
     if teacher_ids.dtype not in _ID_TYPES or not teacher_logprobs.is_floating_point():
