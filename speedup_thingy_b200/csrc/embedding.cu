@@ -77,6 +77,7 @@ embedding_fwd_kernel(const int64_t* __restrict__ ids, long long n, const T* __re
   const int lane = threadIdx.x % tpr, groups = 128 / tpr;
   for (long long t = ((long long)blockIdx.x * groups + threadIdx.x / tpr) * TOKENS_AHEAD; t < n; t += (long long)gridDim.x * groups * TOKENS_AHEAD) {
     long long id[TOKENS_AHEAD];
+    float by[TOKENS_AHEAD];                                        // zero times zero without a row, whatever the scale
 #pragma unroll
     for (int u = 0; u < TOKENS_AHEAD; ++u) {
       id[u] = t + u < n ? ids[t + u] : 0;
@@ -84,6 +85,7 @@ embedding_fwd_kernel(const int64_t* __restrict__ ids, long long n, const T* __re
         if (status && lane == 0 && blockIdx.y == 0) atomicExch(status, RTE_DEV_INDEX_OUT_OF_RANGE);
         id[u] = -1;
       }
+      by[u] = id[u] >= 0 ? scale : 0.f;
     }
     for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) {
       R r[TOKENS_AHEAD];
@@ -91,7 +93,7 @@ embedding_fwd_kernel(const int64_t* __restrict__ ids, long long n, const T* __re
       for (int u = 0; u < TOKENS_AHEAD; ++u) r[u] = id[u] >= 0 ? w[id[u] * pieces + c] : R{};
 #pragma unroll
       for (int u = 0; u < TOKENS_AHEAD; ++u)
-        if (t + u < n) y[(t + u) * pieces + c] = id[u] >= 0 ? pack<T, BYTES>(unpack<T, BYTES>(r[u]), scale) : R{};       // (no product: 0 times infinity)
+        if (t + u < n) y[(t + u) * pieces + c] = pack<T, BYTES>(unpack<T, BYTES>(r[u]), by[u]);
     }
   }
 }
