@@ -10,7 +10,7 @@
 // The sort takes a pass per digit of the id, each stable: a token's place is the number of tokens with a smaller digit, those with its own
 // in CTAs before, in warps before, and in its warp before it.  Up to SORT_ONE tokens are one cluster's, which exchanges its CTAs' counts
 // (digits of up to 8 bits, all passes in one launch).  More are counted by CTAs, and a pass leaves the next digit's counts behind, so that a sort of two digits (of up to 10 bits: tables
-// of up to 2^20 rows) is three launches.
+// of up to 2^20 rows) is three launches.  A few tokens' gradient is one launch: the cluster that sorts them adds their rows too.
 
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -190,11 +190,10 @@ __device__ __forceinline__ int sums_before(int v, int* warp_total) {
 // Up to SORT_ONE tokens by the first cluster, a run of neighbouring tokens per CTA, up to 24 of them a thread; the other clusters fill.  One
 // CTA of 1024 threads took 21 us for 8192 tokens, most of it the rounds of votes on one SM.  Whole gradients, us, launches per digit | one
 // cluster: 16384 x 1024 bf16 of 32768 45 | 37.6, 30000 x 1024 67 | 55, 30000 x 256 of 2000 49 | 38, 45000 x 1024 of 131072 104 | 96.
-__global__ void __cluster_dims__(ONE_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
-embedding_sort_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int passes, int bits, Fill f, int* status) {
-  rte::after_previous_grid();
-  if (blockIdx.x >= ONE_CTAS) return fill(f, blockIdx.x - ONE_CTAS, gridDim.x - ONE_CTAS);
-  constexpr int WARPS = SORT_THREADS / 32, EACH = SORT_ONE / ONE_CTAS / SORT_THREADS, BINS = 1 << ONE_BITS;
+// EACH: tokens of a thread at most.  Ends with a cluster's barrier.
+template <int EACH>
+__device__ __forceinline__ void sort_one(const int64_t* __restrict__ ids, int n, int V, long long padding, const EoScratch& S, int passes, int bits, int* status) {
+  constexpr int WARPS = SORT_THREADS / 32, BINS = 1 << ONE_BITS;
   static_assert(BINS == SORT_THREADS, "a thread per digit");
   __shared__ int base[BINS], count[BINS], warp_total[WARPS];
   __shared__ unsigned short in_warp[WARPS][BINS];
@@ -264,6 +263,12 @@ embedding_sort_kernel(const int64_t* __restrict__ ids, int n, int V, long long p
     }
     cluster.sync();                                                  // (every CTA's places are written, its counts read)
   }
+}
+__global__ void __cluster_dims__(ONE_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
+embedding_sort_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int passes, int bits, Fill f, int* status) {
+  rte::after_previous_grid();
+  if (blockIdx.x >= ONE_CTAS) return fill(f, blockIdx.x - ONE_CTAS, gridDim.x - ONE_CTAS);
+  sort_one<SORT_ONE / ONE_CTAS / SORT_THREADS>(ids, n, V, padding, S, passes, bits, status);
 }
 
 // The first digit's counts of every sort CTA's tokens; the other passes' counts are cleared.
@@ -390,29 +395,18 @@ __device__ __forceinline__ int below(const int* __restrict__ ids, int count, lon
 // Groups of tpr threads: one adds the rows of a range, a piece of the columns per thread.  CTAs behind `range_ctas`: zeros of ZERO_ROWS table
 // rows that no token names, where the sort's launches have not filled the table.
 constexpr int ZERO_ROWS = 64, MIN_TPR = 8;
-template <typename T, int BYTES>
-__global__ void __launch_bounds__(128)
-embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pieces, int tpr, int range, int d, float scale, T* __restrict__ dtable, int range_ctas) {
-  rte::after_previous_grid();
+template <int RANGE> struct Sorted { int ids[128 / MIN_TPR][2 * RANGE + 2], toks[128 / MIN_TPR][2 * RANGE]; };       // of the groups' ranges, and of the next ones
+// By 128 threads, a barrier for all of the CTA in it: the ranges of `block`, the columns of `part` of `parts`.
+template <typename T, int BYTES, int RANGE>
+__device__ __forceinline__ void sum_ranges(Sorted<RANGE>& sorted, int tid, int block, int part, int parts, const T* __restrict__ dy, const EoScratch& S, int n, int V, int pieces,
+                                           int tpr, int range, int d, float scale, T* __restrict__ dtable) {
   using R = typename Raw<T, BYTES>::type;
   using P = Piece<T, BYTES>;
-  __shared__ int ids[128 / MIN_TPR][2 * MAX_RANGE + 2], toks[128 / MIN_TPR][2 * MAX_RANGE];
+  auto& ids = sorted.ids;
+  auto& toks = sorted.toks;
   R* out = reinterpret_cast<R*>(dtable);
-  const int tid = threadIdx.x, groups = 128 / tpr, group = tid / tpr, lane = tid % tpr;
-  if ((int)blockIdx.x >= range_ctas) {
-    int* named = ids[0];                                           // (MAX_RANGE of them)
-    const long long v0 = (long long)ZERO_ROWS * (blockIdx.x - range_ctas);
-    if (tid < ZERO_ROWS) {
-      const int v = (int)min(v0 + tid, (long long)V), at = below(S.id, n, v);
-      named[tid] = at < n && S.id[at] == v;
-    }
-    __syncthreads();
-    for (int r = group; r < ZERO_ROWS && v0 + r < V; r += groups)
-      if (!named[r])
-        for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) out[(v0 + r) * pieces + c] = R{};
-    return;
-  }
-  const long long r0 = (long long)blockIdx.x * groups;
+  const int groups = 128 / tpr, group = tid / tpr, lane = tid % tpr;
+  const long long r0 = (long long)block * groups;
   for (int i = tid; i < groups * (2 * range + 2); i += 128) {
     const int g = i / (2 * range + 2), e = i % (2 * range + 2);
     const long long at = (r0 + g) * range - 1 + e;
@@ -432,12 +426,12 @@ embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pi
   if (last < V && last == id[range] && !(id[0] == last && id[-1] == last)) {      // begins here and goes on:
     if (id[2 * range] != last) {                                   // to be finished here,
       while (id[end] == last) ++end;
-    } else if (lane == 0 && blockIdx.y == 0) {                     // or over a whole range and further, to be joined
+    } else if (lane == 0 && part == 0) {                           // or over a whole range and further, to be joined
       S.joins[atomicAdd(S.join_count, 1)] = make_int2((int)r, last);
     }
   }
   const R* g = reinterpret_cast<const R*>(dy);
-  for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) {
+  for (int c = part * tpr + lane; c < pieces; c += parts * tpr) {
     P acc;
     bool fresh = true, first = begin == 0;
     for (int i0 = begin; i0 < end; i0 += ROWS_AHEAD) {
@@ -468,16 +462,40 @@ embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pi
   }
 }
 
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(128)
+embedding_sum_kernel(const T* __restrict__ dy, EoScratch S, int n, int V, int pieces, int tpr, int range, int d, float scale, T* __restrict__ dtable, int range_ctas) {
+  rte::after_previous_grid();
+  using R = typename Raw<T, BYTES>::type;
+  __shared__ Sorted<MAX_RANGE> sorted;
+  if ((int)blockIdx.x >= range_ctas) {
+    R* out = reinterpret_cast<R*>(dtable);
+    const int tid = threadIdx.x, groups = 128 / tpr, group = tid / tpr, lane = tid % tpr;
+    int* named = sorted.ids[0];                                    // (MAX_RANGE of them)
+    const long long v0 = (long long)ZERO_ROWS * (blockIdx.x - range_ctas);
+    if (tid < ZERO_ROWS) {
+      const int v = (int)min(v0 + tid, (long long)V), at = below(S.id, n, v);
+      named[tid] = at < n && S.id[at] == v;
+    }
+    __syncthreads();
+    for (int r = group; r < ZERO_ROWS && v0 + r < V; r += groups)
+      if (!named[r])
+        for (int c = blockIdx.y * tpr + lane; c < pieces; c += gridDim.y * tpr) out[(v0 + r) * pieces + c] = R{};
+    return;
+  }
+  sum_ranges<T, BYTES, MAX_RANGE>(sorted, threadIdx.x, blockIdx.x, blockIdx.y, gridDim.y, dy, S, n, V, pieces, tpr, range, d, scale, dtable);
+}
+
 // What several ranges have of an id, added in their order: eight warps each take a run of neighbouring ranges, then the warps' sums.
 constexpr int JOIN_WARPS = 8, JOIN_COLUMNS = 128;
+using JoinSums = float[JOIN_WARPS][JOIN_COLUMNS];
+// (CTAs and parts unsigned, as a grid's are: with int the gradient of 131072 x 2048 takes 244 us for 241.)
 template <typename T>
-__global__ void __launch_bounds__(32 * JOIN_WARPS)
-embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __restrict__ dtable) {
-  rte::after_previous_grid();
-  __shared__ float sum[JOIN_WARPS][JOIN_COLUMNS];
+__device__ __forceinline__ void join_ranges(JoinSums& sum, unsigned cta, unsigned ctas, unsigned part, unsigned parts, const EoScratch& S, int n, int range, int d,
+                                            float scale, T* __restrict__ dtable) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int joins = *S.join_count;
-  for (int j = blockIdx.x; j < joins; j += gridDim.x) {
+  for (int j = cta; j < joins; j += ctas) {
     const int2 join = S.joins[j];
     const int r = join.x, v = join.y;
     // how many ranges behind r + 1 begin with the id: leaps of 1024, 32 and one range, a lane each, asked for at once
@@ -496,7 +514,7 @@ embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __re
     if (m > 0) near = begins(m + lane + 1);
     m += __popc(__ballot_sync(0xffffffffu, near)) + 1;             // r + 1 .. r + m
     const int first = int((long long)m * warp / JOIN_WARPS), last = int((long long)m * (warp + 1) / JOIN_WARPS);
-    for (int c0 = blockIdx.y * JOIN_COLUMNS; c0 < d; c0 += gridDim.y * JOIN_COLUMNS) {
+    for (int c0 = part * JOIN_COLUMNS; c0 < d; c0 += parts * JOIN_COLUMNS) {
       const bool mine = tid < JOIN_COLUMNS && c0 + tid < d;
       const float begun = mine ? S.part[((size_t)r * 2 + 1) * d + c0 + tid] : 0.f;
       float a[4] = {0.f, 0.f, 0.f, 0.f};
@@ -517,6 +535,76 @@ embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __re
       __syncthreads();
     }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
+embedding_join_kernel(EoScratch S, int n, int range, int d, float scale, T* __restrict__ dtable) {
+  rte::after_previous_grid();
+  __shared__ JoinSums sum;
+  join_ranges<T>(sum, blockIdx.x, gridDim.x, blockIdx.y, gridDim.y, S, n, range, d, scale, dtable);
+}
+
+// ---------------------------------------------------------------- few tokens: one launch
+// The same three steps by one cluster, a barrier between them, with the same bits; the other clusters write the zeros, of rows that no token
+// names.  Three launches were half of the host's time that such a gradient took beside the autograd engine's own.
+constexpr int FEW = ONE_CTAS * SORT_THREADS, FEW_RANGE = 8, FEW_ROWS = 4096;
+// The first row from r on whose bit is set, `rows` if none is; every warp for itself.
+__device__ __forceinline__ int next_named(const uint32_t* named, int r, int rows) {
+  const int lane = threadIdx.x & 31;
+  for (int w0 = r / 32; w0 * 32 < rows; w0 += 32) {
+    const int w = w0 + lane;
+    uint32_t bits = w * 32 < rows ? named[w] : 0;
+    if (w == r / 32) bits &= 0xffffffffu << (r % 32);
+    const uint32_t some = __ballot_sync(0xffffffffu, bits);
+    if (some == 0) continue;
+    const int first = __ffs(some) - 1;
+    return (w0 + first) * 32 + __ffs(__shfl_sync(0xffffffffu, bits, first)) - 1;
+  }
+  return rows;
+}
+// Zeros in a CTA's share of the rows, run by run between those that a token names.
+__device__ __forceinline__ void zero_unnamed(const int64_t* __restrict__ ids, int n, int V, long long padding, char* table, long long row_bytes, int cta, int ctas) {
+  __shared__ uint32_t named[FEW_ROWS / 32];
+  const int tid = threadIdx.x;
+  const long long each = ((long long)V + ctas - 1) / ctas, last = min((cta + 1) * each, (long long)V);
+  for (long long v0 = cta * each; v0 < last; v0 += FEW_ROWS) {
+    const int rows = (int)min(last - v0, (long long)FEW_ROWS);
+    for (int i = tid; i < FEW_ROWS / 32; i += SORT_THREADS) named[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += SORT_THREADS) {
+      const long long v = ids[i] - v0;
+      if (v >= 0 && v < rows && v + v0 != padding) atomicOr(&named[v / 32], 1u << (v % 32));
+    }
+    __syncthreads();
+    for (int r = 0; r < rows;) {
+      const int to = next_named(named, r, rows);
+      if (to > r) fill({table + (v0 + r) * row_bytes, (to - r) * row_bytes}, 0, 1);
+      r = to + 1;
+    }
+    __syncthreads();
+  }
+}
+template <typename T, int BYTES>
+__global__ void __cluster_dims__(ONE_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
+embedding_few_kernel(const int64_t* __restrict__ ids, int n, int V, long long padding, EoScratch S, int passes, int bits, const T* __restrict__ dy, int pieces, int tpr, int d,
+                     float scale, T* __restrict__ dtable, int* status) {
+  rte::after_previous_grid();
+  const int tid = threadIdx.x;
+  if (blockIdx.x >= ONE_CTAS) return zero_unnamed(ids, n, V, padding, reinterpret_cast<char*>(dtable), (long long)d * sizeof(T), blockIdx.x - ONE_CTAS, gridDim.x - ONE_CTAS);
+  sort_one<1>(ids, n, V, padding, S, passes, bits, status);
+  __shared__ Sorted<FEW_RANGE> sorted[2];                          // (each half of the CTA adds for itself)
+  const int half = tid / 128, rank = blockIdx.x, ranges = (n + FEW_RANGE - 1) / FEW_RANGE, groups = 128 / tpr;
+  const int parts = (pieces + tpr - 1) / tpr, units = (ranges + groups - 1) / groups * parts;
+  for (int u = 2 * rank; u < units; u += 2 * ONE_CTAS) {
+    __syncthreads();
+    sum_ranges<T, BYTES, FEW_RANGE>(sorted[half], tid % 128, (u + half) / parts, (u + half) % parts, parts, dy, S, n, V, pieces, tpr, FEW_RANGE, d, scale, dtable);
+  }
+  if (ranges <= 2) return;
+  static_assert(SORT_THREADS == 32 * JOIN_WARPS, "the join takes all threads");
+  cg::this_cluster().sync();
+  __shared__ JoinSums sum;
+  join_ranges<T>(sum, rank, ONE_CTAS, 0, 1, S, n, FEW_RANGE, d, scale, dtable);
 }
 
 // ---------------------------------------------------------------- launches
@@ -550,9 +638,30 @@ void launch_sum(const void* dy, const EoScratch& s, int n, int V, int d, float s
   }
 }
 
+constexpr int FILL_CTAS = 16 * 148;
+
+// Whether one cluster adds the rows too: up to FEW tokens whose sums are little more than one round of the cluster's (FEW_UNITS runs of 128 threads), and no more
+// table rows than come to 64 a CTA of zeros (named rows end its runs).  The host's time of a gradient's launches 8.5 us -> 3.4; us on the device,
+// three launches | one: 24 x 1518 fp16 of 1206 10.1 | 10.2, 181 x 160 fp32 of 41627 11.8 | 9.8, 128 x 1024 bf16 of 32768 15.5 | 14.0, 16 x 1024 of 32768 13.6 |
+// 13.9, 2048 x 8 of 131072 16.6 | 18.0; beyond the rule 500 x 1024 of 32768 17.1 | 23.7, 2048 x 8 of 10^6 18 | 50.
+constexpr int FEW_UNITS = 24;
+template <typename T, int BYTES>
+bool launch_few(const int64_t* ids, int n, const void* dy, const EoScratch& s, int V, int d, float scale, long long padding, void* dtable, int* status, cudaStream_t st) {
+  if (n > FEW || V > 64 * FILL_CTAS) return false;
+  static_assert(FEW < 8192, "ranges of FEW_RANGE rows");
+  const int pieces = pieces_of<T, BYTES>(d), tpr = max(threads_per_row(pieces), MIN_TPR), range_ctas = rte::ceil_div(rte::ceil_div(n, FEW_RANGE), 128 / tpr);
+  if ((long long)range_ctas * rte::ceil_div(pieces, tpr) > FEW_UNITS) return false;
+  const Digits dg = digits_of(V, ONE_BITS);
+  // a CTA of zeros per 32 KB or 64 rows
+  const long long zeros = max((long long)V * d * (int)sizeof(T) / 32768, (long long)V / 64);
+  const int fills = (int)min((zeros / ONE_CTAS + 1) * ONE_CTAS, (long long)FILL_CTAS);
+  rte::launch(embedding_few_kernel<T, BYTES>, ONE_CTAS + fills, SORT_THREADS, 0, st, ids, n, V, padding, s, dg.passes, dg.bits, static_cast<const T*>(dy), pieces, tpr, d, scale,
+              static_cast<T*>(dtable), status);
+  return true;
+}
+
 // id and tok sorted; `table` (NULL: not) filled with zeros on the way, by FILL_CTAS CTAs in each launch (33333 x 770 fp32 of 50257, the whole
 // gradient, 1 | 2 | 7 | 16 of them per SM: 91 | 78 | 72 | 70 us), a pass's share twice that of the count, which is done sooner.
-constexpr int FILL_CTAS = 16 * 148;
 void launch_sort(const int64_t* ids, int n, int V, long long padding, const EoScratch& s, char* table, long long table_bytes, int* status, cudaStream_t st) {
   const bool one = n <= SORT_ONE;
   const Digits dg = digits_of(V, one ? ONE_BITS : SORT_BITS);
@@ -630,6 +739,14 @@ extern "C" int rte_embedding_bwd(const int64_t* ids, int64_t n, const void* dy, 
   // they are looked for beside the sums (us, filled ahead | looked for: 33333 x 770 fp32 of 50257 69 | 89, 60000 x 2048 bf16 of 131072 188 | 186, 131072 x
   // 2048 of 131072 241 | 244).
   const bool fill_ahead = n <= V;
+  bool few = false;
+#define CALL(T, B) few = launch_few<T, B>(ids, (int)n, dy, s, V, d, scale, padding_idx, dtable, status, ST(stream))
+  BY_PIECE(type, bytes, CALL);
+#undef CALL
+  if (few) {
+    RTE_LAUNCH_CHECK();
+    return RTE_OK;
+  }
   launch_sort(ids, (int)n, V, padding_idx, s, fill_ahead ? static_cast<char*>(dtable) : nullptr, (long long)V * d * (type == RTE_TYPE_F32 ? 4 : 2), status, ST(stream));
 #define CALL(T, B) launch_sum<T, B>(dy, s, (int)n, V, d, scale, dtable, fill_ahead, ST(stream))
   BY_PIECE(type, bytes, CALL);

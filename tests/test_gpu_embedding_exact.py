@@ -49,3 +49,14 @@ def test_runs_that_end_about_a_range(n):
     order = torch.randperm(n, device=DEV, generator=torch.Generator(device=DEV).manual_seed(n))
     for v in (ids, ids[order]):
         check(v, len(runs) + 2, 9, seed=n)
+
+
+@pytest.mark.parametrize("kind", ["zipf", "same", "distinct", "ascending", "ends", "random"])
+# few tokens are added in one launch: its limits of tokens, columns and rows, and rows that share 16 bytes
+@pytest.mark.parametrize("n, V, d", [(1, 1, 1), (2, 3, 5), (16, 300, 33), (17, 40, 2048), (64, 64 * 2368, 3), (64, 64 * 2368 + 1, 3), (128, 5000, 512), (136, 5000, 512), (2047, 2000, 8),
+                                     (2048, 100000, 7), (2049, 100000, 7), (2048, 9, 32), (1000, 151000, 31), (8, 30000, 770), (300, 4097, 130)])
+def test_few_tokens(n, V, d, kind):
+    ids = some_ids(kind, n, V)
+    check(ids, V, d, seed=n)
+    check(ids, V, d, seed=n + 1, padding=int(ids[0]))
+    check(ids, V, d, seed=n + 2, padding=V - 1)
