@@ -29,7 +29,8 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int TS_MAX_LIST = RTE_TOKEN_LIST_MAX;
-// Forward's CTAs on an SM: 24 to 40 warps are in flight, a thread has 80, 48 or 64 registers.
+// Forward's CTAs on an SM: 24 to 40 warps are in flight, a thread has 80, 48 or 64 registers.  (With 48, lists spill up to 260 bytes; ten CTAs | eight with 64
+// registers, us, 32 alternatives of 2048 bf16 columns: 256 rows 6.6 | 6.2, 1000 10.8 | 8.8, 2900 19.3 | 19.9, none: 2.7 | 2.8, 4.65 | 4.25, 7.9 | 8.3.)
 __host__ __device__ constexpr int min_ctas(int nt, int u) { return nt == 32 ? 24 : nt == 256 ? 4 : u == 4 ? 10 : 8; }
 constexpr int TS_MAX_V = 0x7fffff00;           // (columns and what is added to them stay within an int)
 constexpr float LN2 = 0.693147180559945309f;
@@ -39,8 +40,8 @@ constexpr float LOW = -1e30f;                  // the least logit that enters an
 constexpr float MIN_T = 1e-6f, MAX_T = 1e6f;   // temperatures: LOW is then within fp32 after scaling
 // Distillation above this temperature has its sums and its listed columns' gradients in 64 bits: the loss is T^2 times a divergence that falls
 // as T^-2, so that an error of 1e-7 in a row's logarithm, fp32's, is one of T^2 1e-7 in a loss of order one.  The second pass over the row is bound
-// by the fp64 pipe (8192 x 32768 bf16, 64 listed, us forward | backward at T = 8 and above it: 104 | 170 and 502 | 236, with the rest 125 | 168 and
-// 629 | 229), which is why lower temperatures, where that error is below 1e-5, go without.
+// by instructions (71 a logit, 81 % of the issue slots; the fp64 pipe 41 %): 8192 x 32768 bf16, 64 listed, us forward | backward at T = 8 and above it
+// 104 | 170 and 502 | 236, with the rest 125 | 168 and 629 | 229, which is why lower temperatures, where that error is below 1e-5, go without.
 constexpr float HOT_T = 8.f;
 
 __device__ __forceinline__ float exp2_fast(float t) {            // relative error up to 2^-22.5, 0 below -126
@@ -1073,8 +1074,8 @@ int pieces_of(const void* x, int type, long long ld, int V) {
 }
 
 // A row of at most one tile of 32 or 128 threads is one CTA of them; longer ones are walked by 256.
-// Forward, who walks a row.  Many short rows: a warp each (us, 8192 x 2048 bf16, warp | 128 threads: 11.0 | 20, with 32 alternatives 39 | 60;
-// 16384 x 5000 41 | 57, 16384 x 9001 with 50 181 | 225, 16384 x 16000 108 | 98; 256 x 2048: 6.2 | 4.8).  Many long ones: 128 threads (8192 x 32768 bf16, warp | 128 | 256 | 512: 119 | 97 | 105 | 151), eight loads each for
+// Forward, who walks a row.  Many short rows: a warp each (us, 8192 x 2048 bf16, warp | 128 threads: 10.7 | 18.5, with 32 alternatives 31 | 49;
+// 16384 x 5000 41 | 57, with 32 93 | 117; 16384 x 9001 with 50 168 | 187; 16384 x 16000 108 | 98, with 50 222 | 186; 256 x 2048 3.4 | 2.7, with 32 8.3 | 6.5).  Many long ones: 128 threads (8192 x 32768 bf16, warp | 128 | 256 | 512: 119 | 97 | 105 | 151), eight loads each for
 // scores, four for distillation, which has more to keep (2000 x 131072 with 64 alternatives, 4 | 8: 133 | 118; 8192 x 32768 distilled 127 | 134).
 // Few long ones, where latency counts: 256 threads, eight loads each (1 x 50257 with 20 alternatives, 128 x 4 | 256 x 4 | 256 x 8: 12.8 | 10.7 | 9.2).
 constexpr int MANY_SHORT = 20 * 148, MANY_LONG = 2 * 148;
