@@ -524,7 +524,9 @@ bool differentiable(const Tensor& t) { return (at::GradMode::is_enabled() && t.r
 // A gradient that cannot be differentiated again: where a graph of it is asked for (create_graph), it has an edge to each tensor that it
 // depends on, which raises when it is walked.
 struct FirstDerivative : Function<FirstDerivative> {
-  static variable_list forward(AutogradContext*, const Tensor& dx, const Tensor&, const Tensor&, const Tensor&, const Tensor&) { return {dx}; }
+  static variable_list forward(AutogradContext*, const Tensor& dx, const Tensor&, const Tensor&, const Tensor&, const Tensor&) {
+    return {dx.detach()};                    // (an input itself would come out as a view, which cannot be changed in place)
+  }
   static variable_list backward(AutogradContext*, variable_list) {
     TORCH_CHECK(false, "rte_b200: trying to differentiate twice an operator that has first derivatives only");
   }

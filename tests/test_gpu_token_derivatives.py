@@ -54,3 +54,20 @@ def test_second_derivatives_are_refused(name):
     for of in (g,) if name == "embedding" else (x, g):           # (a table's gradient does not depend on the table)
         with pytest.raises(RuntimeError, match="differentiate twice"):
             torch.autograd.grad([(dx * dx).sum() + (x * x).sum() + (g * g).sum()], [of], retain_graph=True)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_gradient_with_a_graph_can_be_changed_in_place(name):
+    x = inputs()[0].requires_grad_()
+    want, = torch.autograd.grad([CALLS[name](x).sum()], [x])
+    for how in ("grad", "backward"):
+        if how == "grad":
+            dx, = torch.autograd.grad([CALLS[name](x).sum()], [x], create_graph=True)
+        else:
+            CALLS[name](x).sum().backward(create_graph=True)
+            dx = x.grad
+        with torch.no_grad():
+            dx.mul_(0.5)
+        dx.detach_()
+        assert torch.equal(dx, 0.5 * want) and not dx.requires_grad
+        x.grad = None
