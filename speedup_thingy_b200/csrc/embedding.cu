@@ -573,8 +573,8 @@ __device__ __forceinline__ void zero_unnamed(const int64_t* __restrict__ ids, in
     for (int i = tid; i < FEW_ROWS / 32; i += SORT_THREADS) named[i] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += SORT_THREADS) {
-      const long long v = ids[i] - v0;
-      if (v >= 0 && v < rows && v + v0 != padding) atomicOr(&named[v / 32], 1u << (v % 32));
+      const long long v = ids[i];
+      if (v >= v0 && v < v0 + rows && v != padding) atomicOr(&named[(v - v0) / 32], 1u << ((v - v0) % 32));
     }
     __syncthreads();
     for (int r = 0; r < rows;) {
